@@ -1,0 +1,83 @@
+// Copies of pages of the paged KV cache: a fork's private copy of its last, partly filled page, compaction of the pool, the
+// move into another cache, and clearing. A page is 16 tokens of every layer and kv head: in the cache tensors
+// [layers][blocks][n_kv][16 * 128] it is one contiguous slab of n_kv * 2048 elements per layer, in K and in V.
+//
+// Nothing is computed: the floor is each page read once and written once. The page numbers travel in the launch's own
+// arguments, up to PAIRS of them, so a call needs no copy to the device, no buffer that has to outlive it, and can be captured.
+//
+// No reference counterpart (vLLM is a README bullet in the reference, README.md:73).
+#include "llm_common.h"
+
+using namespace klm_llm;
+
+namespace {
+
+constexpr int PAIRS = 256;
+struct PagePairs {
+  int src[PAIRS], dst[PAIRS];      // src < 0: clear dst
+};
+
+struct PageArgs {
+  const char *ks, *vs;
+  char *kd, *vd;
+  size_t slab;                     // bytes of one page of one layer
+  size_t src_layer, dst_layer;     // bytes from one layer to the next
+  int chunks;                      // blocks per slab
+};
+
+constexpr int PER_BLOCK = 16384;   // bytes a block moves: 4 x 16 bytes a thread
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(PageArgs a, PagePairs p) {
+  const int pair = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, layer = blockIdx.y;
+  const int src = p.src[pair], dst = p.dst[pair];
+  const bool v = blockIdx.z != 0;
+  const size_t at = (size_t)chunk * PER_BLOCK + threadIdx.x * 16;
+  const char* s = (v ? a.vs : a.ks) + (size_t)layer * a.src_layer + (size_t)(src < 0 ? 0 : src) * a.slab;
+  char* d = (v ? a.vd : a.kd) + (size_t)layer * a.dst_layer + (size_t)dst * a.slab;
+  uint4 r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r[j] = uint4{0, 0, 0, 0};
+    if (src >= 0 && at + j * 4096 < a.slab) r[j] = *reinterpret_cast<const uint4*>(s + at + j * 4096);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (at + j * 4096 < a.slab) *reinterpret_cast<uint4*>(d + at + j * 4096) = r[j];
+}
+
+}  // namespace
+
+extern "C" {
+
+int klm_copy_pages(const void* k_src, const void* v_src, void* k_dst, void* v_dst, const int32_t* pairs, int n, int layers,
+                   int src_blocks, int dst_blocks, int n_kv, int elem_size, void* stream) {
+  if (n < 0 || layers <= 0 || layers > 65535 || src_blocks <= 0 || dst_blocks <= 0 || n_kv <= 0) return KLM_ERR_SHAPE;
+  if ((elem_size != 1 && elem_size != 2) || (n > 0 && !pairs) || !k_src || !v_src || !k_dst || !v_dst) return KLM_ERR_ARG;
+  if (!aligned16(k_src) || !aligned16(v_src) || !aligned16(k_dst) || !aligned16(v_dst)) return KLM_ERR_ALIGN;
+  for (int i = 0; i < n; ++i)
+    if (pairs[2 * i] >= src_blocks || pairs[2 * i + 1] < 0 || pairs[2 * i + 1] >= dst_blocks) return KLM_ERR_ARG;
+  PageArgs a;
+  a.ks = (const char*)k_src;
+  a.vs = (const char*)v_src;
+  a.kd = (char*)k_dst;
+  a.vd = (char*)v_dst;
+  a.slab = (size_t)n_kv * BLK_ELEMS * elem_size;
+  a.src_layer = a.slab * src_blocks;
+  a.dst_layer = a.slab * dst_blocks;
+  const size_t chunks = (a.slab + PER_BLOCK - 1) / PER_BLOCK;
+  if (chunks > 65535) return KLM_ERR_SHAPE;
+  a.chunks = (int)chunks;
+  for (int at = 0; at < n; at += PAIRS) {
+    const int m = n - at < PAIRS ? n - at : PAIRS;
+    PagePairs p;
+    for (int i = 0; i < PAIRS; ++i) {
+      p.src[i] = i < m ? pairs[2 * (at + i)] : -1;
+      p.dst[i] = i < m ? pairs[2 * (at + i) + 1] : 0;
+    }
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(m * a.chunks), layers, 2), dim3(256), 0, static_cast<hipStream_t>(stream), a, p);
+    if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
+  }
+  return KLM_OK;
+}
+
+}  // extern "C"

@@ -1,4 +1,5 @@
-"""LLM serving ops: RMSNorm, SwiGLU, RoPE + paged-cache write, paged attention (decode, prefill).
+"""LLM serving ops: RMSNorm, SwiGLU, RoPE + paged-cache write, paged attention (decode, prefill), the same with a sliding
+window and sinks, copies of cache pages, rules on logits with the greedy choice.
 
 On a GPU every call runs the hand-written gfx950 kernel of ``csrc/llm_*.hip`` (ctypes, current
 torch stream, no allocation inside the launcher, so the calls can be captured into a hipGraph);
@@ -9,12 +10,15 @@ No reference counterpart (vLLM is a README bullet in the reference, README.md:73
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
-from . import KlmOpsError, _check, load
+from . import KlmOpsError, _check, _on_device, load
 from . import _stream_of as _stream
 from . import ref
 
@@ -56,6 +60,13 @@ def _lib():
         lib.klm_gemm_bf16_swiglu.restype = i
         for n in ("klm_mid_linear_plan", "klm_mid_linear", "klm_mid_linear_w8", "klm_mid_epilogue", "klm_rope_cache_from_partials",
                   "klm_mid_linear_swiglu"):
+            getattr(lib, n).restype = i
+        lib.klm_window_attn_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, vp]
+        lib.klm_window_attn_prefill.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, i, vp]
+        lib.klm_copy_pages.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp]
+        lib.klm_logits_slices.argtypes = [i]
+        lib.klm_choose_tokens.argtypes = [vp, i, i64, i, i, i, vp, i, vp, i, vp, vp, vp, vp, vp, vp, vp, i, vp, i, i, vp, vp, vp, vp, vp, vp]
+        for n in ("klm_window_attn_decode", "klm_window_attn_prefill", "klm_copy_pages", "klm_logits_slices", "klm_choose_tokens"):
             getattr(lib, n).restype = i
         for n in ("klm_rmsnorm", "klm_silu_mul", "klm_rope_cache", "klm_paged_attn_decode", "klm_paged_attn_prefill",
                   "klm_skinny_linear"):
@@ -591,3 +602,310 @@ def paged_attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                                        int(variant), _kv8(k_cache), _stream(q))
     _check(rc, f"klm_paged_attn_prefill(tiles={tiles.shape[0]})")
     return out
+
+
+# ------------------------------------------------------------------ sliding window and sinks
+_HERE = contextlib.nullcontext()
+
+
+def _launch_on(t: torch.Tensor):
+    """The device that a launch for `t` has to be made on, where it is not the current one."""
+    return _HERE if t.device.index == torch.cuda.current_device() else _on_device(t)
+
+
+def _same_device(what: str, t: torch.Tensor, *others) -> None:
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise KlmOpsError(f"{what}: tensors on {t.device} and {o.device}")
+
+
+_FAR = 1 << 30          # a window or sinks beyond any context; keeps the kernels' 32-bit positions from running over
+
+
+def _check_window(what: str, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out) -> Tuple[int, int, int]:
+    """-> blocks of the cache, window, sinks."""
+    n_kv = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    nb = _check_caches(k_cache, v_cache, n_kv)
+    if nb < 1 or n_kv < 1 or n_q < 1 or n_q % n_kv:
+        raise KlmOpsError(f"{what}: {n_q} query heads, cache {tuple(k_cache.shape)}")
+    if q.dim() != 2 or q.shape[1] < n_q * HEAD_DIM or q.stride(1) != 1 or (q.shape[0] > 1 and q.stride(0) < n_q * HEAD_DIM):
+        raise KlmOpsError(f"{what}: q {tuple(q.shape)} strides {q.stride()} for {n_q} heads")
+    if block_tables.dim() != 2 or block_tables.shape[1] < 1:
+        raise KlmOpsError(f"{what}: block_tables {tuple(block_tables.shape)}")
+    if int(window) < 1 or int(sinks) < 0:
+        raise KlmOpsError(f"{what}: window {window} (at least 1: the token itself), sinks {sinks}")
+    if not 0.0 < float(scale) < float("inf"):
+        raise KlmOpsError(f"{what}: scale {scale}")
+    if out is not None and (tuple(out.shape) != (q.shape[0], n_q * HEAD_DIM) or out.dtype != q.dtype or not out.is_contiguous()):
+        raise KlmOpsError(f"{what}: out {tuple(out.shape)} {out.dtype}")
+    _same_device(what, q, k_cache, v_cache, block_tables, out)
+    return nb, min(int(window), _FAR), min(int(sinks), _FAR)
+
+
+def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                             ctx_lens: torch.Tensor, scale: float, n_q: int, window: int, sinks: int = 0,
+                             out: Optional[torch.Tensor] = None, num_splits: int = 0,
+                             workspace: Optional[DecodeWorkspace] = None) -> torch.Tensor:
+    """`paged_attn_decode` of a model whose tokens see the last `window` tokens (their own among them) and the first `sinks`
+    of the context: sequence b's token stands at position ctx_lens[b] - 1 and sees key j <= that with
+    ``j > position - window or j < sinks``.
+
+    Pages between the sinks and the window are not looked at: their table entries may hold anything. An entry outside the
+    cache (-1) is no page and its tokens are not seen, nor are tokens beyond the table. A sequence that sees nothing (length
+    0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `num_splits` 0: chosen from the shapes.
+    `workspace`: the splits' scratch, for calls that must not share it with the allocator; one per stream."""
+    what = "paged_attn_decode_window"
+    nb, window, sinks = _check_window(what, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out)
+    B, width = block_tables.shape
+    n_kv = k_cache.shape[1]
+    if q.shape[0] != B or ctx_lens.shape != (B,):
+        raise KlmOpsError(f"{what}: q {tuple(q.shape)}, ctx_lens {tuple(ctx_lens.shape)} for {B} table rows")
+    if not 0 <= int(num_splits) <= 256:
+        raise KlmOpsError(f"{what}: num_splits {num_splits}")
+    _same_device(what, q, ctx_lens)
+    if not q.is_cuda:
+        o = ref.window_attn_decode(q[:, : n_q * HEAD_DIM], k_cache, v_cache, block_tables, ctx_lens, scale, window, sinks)
+        return o if out is None else out.copy_(o)
+    _bf16(q)
+    _i32(block_tables, ctx_lens)
+    if out is None:
+        out = torch.empty((B, n_q * HEAD_DIM), dtype=q.dtype, device=q.device)
+    if B == 0:
+        return out
+    splits = int(num_splits) or pick_splits(B, n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
+    part_o = part_ml = None
+    if splits > 1:
+        if workspace is None:
+            workspace = DecodeWorkspace(B, n_q, splits, q.device)
+        if workspace.max_batch < B or workspace.n_q != n_q or workspace.max_splits < splits or workspace.tmp_o.device != q.device:
+            raise KlmOpsError(f"{what}: workspace too small")
+        part_o, part_ml = workspace.tmp_o.data_ptr(), workspace.tmp_ml.data_ptr()
+    with _launch_on(q):
+        rc = _lib().klm_window_attn_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+                                           ctx_lens.data_ptr(), out.data_ptr(), part_o, part_ml, B, q.stride(0), n_q, n_kv, width, nb,
+                                           window, sinks, splits, float(scale), _kv8(k_cache), _stream(q))
+    _check(rc, f"klm_window_attn_decode(B={B},window={window},sinks={sinks},splits={splits})")
+    return out
+
+
+def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                              seq_info: torch.Tensor, scale: float, n_q: int, window: int, sinks: int = 0,
+                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`paged_attn_prefill` with a sliding window and sinks (see `paged_attn_decode_window`): the queries of sequence s are the
+    last q_len tokens of a context of ctx_len that is in the cache already; seq_info int32 [S, 3] = (q_start, q_len, ctx_len).
+
+    No table of tiles: the kernel finds its work in `seq_info`, so nothing is computed on the host from the lengths and a
+    captured call may be replayed with others. The sequences' rows must not overlap. Rows of no sequence (padding, or one
+    with q_len <= 0 or ctx_len < q_len) stay as they are in a given `out` and are zero otherwise."""
+    what = "paged_attn_prefill_window"
+    nb, window, sinks = _check_window(what, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out)
+    S, width = block_tables.shape
+    n_kv = k_cache.shape[1]
+    T = q.shape[0]
+    if tuple(seq_info.shape) != (S, 3):
+        raise KlmOpsError(f"{what}: seq_info {tuple(seq_info.shape)} for {S} table rows")
+    _same_device(what, q, seq_info)
+    if not q.is_cuda:
+        return ref.window_attn_prefill(q[:, : n_q * HEAD_DIM], k_cache, v_cache, block_tables, seq_info, scale, window, sinks, out)
+    _bf16(q)
+    _i32(block_tables, seq_info)
+    if out is None:
+        out = torch.zeros((T, n_q * HEAD_DIM), dtype=q.dtype, device=q.device)
+    if T == 0 or S == 0:
+        return out
+    with _launch_on(q):
+        rc = _lib().klm_window_attn_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+                                            seq_info.data_ptr(), out.data_ptr(), T, S, q.stride(0), n_q, n_kv, width, nb,
+                                            window, sinks, float(scale), 2, _kv8(k_cache), _stream(q))
+    _check(rc, f"klm_window_attn_prefill(T={T},S={S},window={window},sinks={sinks})")
+    return out
+
+
+# ------------------------------------------------------------------ pages of a cache
+def _page_shape(k: torch.Tensor, v: torch.Tensor) -> Tuple[int, int, int]:
+    """(layers, blocks, n_kv) of a cache [layers, blocks, n_kv, 16, 128] / [.., 128, 16], or of one layer of it."""
+    if k.dim() == 4 and v.dim() == 4:
+        k, v = k[None], v[None]
+    if k.dim() != 5 or tuple(k.shape[3:]) != (BLOCK, HEAD_DIM) or tuple(v.shape) != (*k.shape[:3], HEAD_DIM, BLOCK) or k.dtype != v.dtype or \
+            not k.is_contiguous() or not v.is_contiguous() or min(k.shape) < 1:
+        raise KlmOpsError(f"copy_pages: cache shapes K {tuple(k.shape)} {k.dtype} V {tuple(v.shape)} {v.dtype}")
+    return int(k.shape[0]), int(k.shape[1]), int(k.shape[2])
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.device == b.device and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and \
+        b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs: Sequence[Tuple[int, int]],
+               k_src: Optional[torch.Tensor] = None, v_src: Optional[torch.Tensor] = None) -> None:
+    """Pages ``src -> dst`` of `pairs`, in every layer, K and V; ``src = -1`` clears the page to zeros.
+
+    `k_cache` / `v_cache`: the whole cache [layers, blocks, n_kv, ..] or one layer [blocks, n_kv, ..], bf16 or e4m3. With
+    `k_src` / `v_src` the pages come from another cache of the same layers, heads and type (any number of blocks): the move
+    into a smaller or larger one. `pairs` are host numbers; the call copies nothing to the device and does not wait. All pairs
+    happen at once, so a page may be written by one pair only and may not be read by another; a pair of a page and itself
+    does nothing. A captured call repeats these pairs."""
+    if (k_src is None) != (v_src is None):
+        raise KlmOpsError("copy_pages: k_src and v_src go together")
+    L, nb, n_kv = _page_shape(k_cache, v_cache)
+    same = k_src is None
+    if same:
+        k_src, v_src, src_nb = k_cache, v_cache, nb
+    else:
+        sl, src_nb, skv = _page_shape(k_src, v_src)
+        if (sl, skv) != (L, n_kv) or k_src.dtype != k_cache.dtype:
+            raise KlmOpsError(f"copy_pages: from {tuple(k_src.shape)} {k_src.dtype} to {tuple(k_cache.shape)} {k_cache.dtype}")
+        same = k_src.data_ptr() == k_cache.data_ptr() and v_src.data_ptr() == v_cache.data_ptr() and src_nb == nb
+        if not same and any(_overlap(a, b) for a in (k_src, v_src) for b in (k_cache, v_cache)):
+            raise KlmOpsError("copy_pages: the two caches share memory")
+    if _overlap(k_cache, v_cache):
+        raise KlmOpsError("copy_pages: K and V share memory")
+    _same_device("copy_pages", k_cache, v_cache, k_src, v_src)
+    elem = k_cache.element_size()
+    if k_cache.is_cuda:
+        _kv8(k_cache)
+    p = np.asarray(pairs, dtype=np.int64).reshape(-1, 2)
+    if not len(p):
+        return
+    src, dst = p[:, 0], p[:, 1]
+    if src.min() < -1 or src.max() >= src_nb or dst.min() < 0 or dst.max() >= nb:
+        raise KlmOpsError(f"copy_pages: a pair outside the caches ({src_nb} and {nb} blocks; -1 clears)")
+    if len(np.unique(dst)) != len(dst):
+        raise KlmOpsError("copy_pages: a page is written twice")
+    if same:
+        p = p[src != dst]
+        if len(np.intersect1d(p[:, 0], dst)):
+            raise KlmOpsError("copy_pages: a page is written by one pair and read by another")
+        if not len(p):
+            return
+    if not k_cache.is_cuda:
+        ref.copy_pages(k_cache, v_cache, p, k_src, v_src)
+        return
+    p = np.ascontiguousarray(p, dtype=np.int32)
+    with _launch_on(k_cache):
+        rc = _lib().klm_copy_pages(k_src.data_ptr(), v_src.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p.ctypes.data, len(p),
+                                   L, src_nb, nb, n_kv, elem, _stream(k_cache))
+    _check(rc, f"klm_copy_pages(pairs={len(p)},layers={L})")
+
+
+# ------------------------------------------------------------------ rules on logits
+@dataclass
+class LogitRules:
+    """What `choose_tokens` does to rows of logits. R sets of rules:
+
+    history int32 [R, n]      token ids, the prompt's first, then the output's; prompt_lens, lens int32 [R]: where they end
+    repetition, frequency, presence fp32 [R]     the penalties (neutral: 1, 0, 0)
+    bias_ids int32, bias_values fp32 [R, k]      added to those tokens (id -1: unused entry; a token twice: the later counts)
+    mask int32 [M, words]     bit v % 32 of word v // 32 set: token v is allowed
+    mask_rows int32 [R]       each set's mask (-1: none); without it set r uses mask r
+    rows int32 [B]            the set that each row of logits follows (-1: none); without it row b follows set b
+
+    Ids outside the vocabulary are ignored. The tensors are read when the call runs: they may be changed between calls and
+    between replays of a captured one."""
+    history: torch.Tensor
+    prompt_lens: torch.Tensor
+    lens: torch.Tensor
+    repetition: torch.Tensor
+    frequency: torch.Tensor
+    presence: torch.Tensor
+    bias_ids: Optional[torch.Tensor] = None
+    bias_values: Optional[torch.Tensor] = None
+    mask: Optional[torch.Tensor] = None
+    mask_rows: Optional[torch.Tensor] = None
+    rows: Optional[torch.Tensor] = None
+
+    def check(self, B: int, vocab_end: int, device) -> None:
+        R = self.lens.shape[0]
+        i32, f32 = torch.int32, torch.float32
+
+        def bad(name: str, t: torch.Tensor, shape, dtype) -> bool:
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+                raise KlmOpsError(f"LogitRules: {name} must be contiguous {dtype} {list(shape)} on {device}, is {t.dtype} "
+                                  f"{list(t.shape)} on {t.device}")
+            return False
+
+        if self.history.dim() != 2:
+            raise KlmOpsError("LogitRules: history must be [R, n]")
+        bad("history", self.history, (R, self.history.shape[1]), i32)
+        bad("prompt_lens", self.prompt_lens, (R,), i32)
+        bad("lens", self.lens, (R,), i32)
+        for name in ("repetition", "frequency", "presence"):
+            bad(name, getattr(self, name), (R,), f32)
+        if (self.bias_ids is None) != (self.bias_values is None):
+            raise KlmOpsError("LogitRules: bias_ids and bias_values go together")
+        if self.bias_ids is not None:
+            if self.bias_ids.dim() != 2:
+                raise KlmOpsError("LogitRules: bias_ids must be [R, k]")
+            bad("bias_ids", self.bias_ids, (R, self.bias_ids.shape[1]), i32)
+            bad("bias_values", self.bias_values, tuple(self.bias_ids.shape), f32)
+        if self.mask is not None:
+            if self.mask.dim() != 2 or self.mask.shape[1] * 32 < vocab_end:
+                raise KlmOpsError(f"LogitRules: mask {tuple(self.mask.shape)} has no bit for each of {vocab_end} tokens")
+            bad("mask", self.mask, tuple(self.mask.shape), i32)
+            if self.mask_rows is not None:
+                bad("mask_rows", self.mask_rows, (R,), i32)
+            elif self.mask.shape[0] < R:
+                raise KlmOpsError(f"LogitRules: {self.mask.shape[0]} masks for {R} sets of rules and no mask_rows")
+        elif self.mask_rows is not None:
+            raise KlmOpsError("LogitRules: mask_rows without a mask")
+        if self.rows is not None:
+            bad("rows", self.rows, (B,), i32)
+        elif R < B:
+            raise KlmOpsError(f"LogitRules: {R} sets of rules for {B} rows of logits and no `rows`")
+
+
+def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, first_token: int = 0,
+                  out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Greedy choice under `rules` -> (token ids int64 [B], their processed logits fp32 [B]).
+
+    For token v of a row: ``x = seen ? (x > 0 ? x / repetition : x * repetition) : x`` where `seen` is: v is in the history;
+    ``x -= frequency * c`` and, where c > 0, ``x -= presence``, c being how often v is in the history's output part;
+    ``x += bias``; a token that the mask does not allow becomes -inf. Each step is rounded to fp32 by itself. The choice is the allowed token
+    of the largest value, the lowest id among equals (NaN counts as largest, as in torch.argmax), -1 where none is allowed.
+
+    `logits` bf16 or fp32 [B, V], rows may be further apart than V; `first_token`: the id of column 0 (a rank's slice of a
+    vocabulary; history, biases, masks and the returned ids are in the whole vocabulary's numbers). `out` fp32 [B, V]: receives
+    the processed logits. `logits` is left as it is (`out` may be `logits` itself if that is contiguous fp32)."""
+    what = "choose_tokens"
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.shape[1] < 1 or \
+            (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise KlmOpsError(f"{what}: logits {tuple(logits.shape)} {logits.dtype} strides {logits.stride()}")
+    B, V = logits.shape
+    if first_token < 0 or first_token + V > 2 ** 31 - 1:
+        raise KlmOpsError(f"{what}: first_token {first_token}")
+    if out is not None:
+        if tuple(out.shape) != (B, V) or out.dtype != torch.float32 or not out.is_contiguous() or out.device != logits.device:
+            raise KlmOpsError(f"{what}: out must be contiguous fp32 {[B, V]} on {logits.device}")
+        if _overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and logits.dtype == torch.float32 and logits.is_contiguous()):
+            raise KlmOpsError(f"{what}: out overlaps logits")
+    if rules is not None:
+        rules.check(B, first_token + V, logits.device)
+    if not logits.is_cuda:
+        y, ids, best = ref.choose_tokens(logits, rules, first_token)
+        if out is not None:
+            out.copy_(y)
+        return ids, best
+    ids = torch.empty(B, dtype=torch.int64, device=logits.device)
+    best = torch.empty(B, dtype=torch.float32, device=logits.device)
+    if B == 0:
+        return ids, best
+    lib = _lib()
+    part = torch.empty((B, lib.klm_logits_slices(V)), dtype=torch.int64, device=logits.device)
+    r = rules
+
+    def ptr(t: Optional[torch.Tensor]):
+        return None if t is None else t.data_ptr()
+
+    if r is None:
+        args = (None, 0, None, 0, None, None, None, None, None, None, None, 0, None, 0, 0, None)
+    else:
+        args = (ptr(r.rows), r.lens.shape[0], r.history.data_ptr(), r.history.shape[1], r.prompt_lens.data_ptr(), r.lens.data_ptr(),
+                r.repetition.data_ptr(), r.frequency.data_ptr(), r.presence.data_ptr(), ptr(r.bias_ids), ptr(r.bias_values),
+                0 if r.bias_ids is None else r.bias_ids.shape[1], ptr(r.mask), 0 if r.mask is None else r.mask.shape[0],
+                0 if r.mask is None else r.mask.shape[1], ptr(r.mask_rows))
+    with _launch_on(logits):
+        rc = lib.klm_choose_tokens(logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0) if B > 1 else V, B, V, first_token, *args,
+                                   ptr(out), part.data_ptr(), ids.data_ptr(), best.data_ptr(), _stream(logits))
+    _check(rc, f"klm_choose_tokens(B={B},V={V})")
+    return ids, best
