@@ -204,8 +204,8 @@ int klm_copy_pages(const void* k_src, const void* v_src, void* k_dst, void* v_ds
 
 // Rules on logits and the greedy choice (llm_logits.hip): logits[B][V] bf16 or fp32, `first` the token id of column 0, R sets
 // of rules, rows[B] the set of each row (null: its own number; outside 0 .. R - 1: none). out [B][V] fp32 or null;
-// part: 8 * B * klm_logits_slices(V) bytes of scratch; ids[B], best[B] the choice and its value.
-int klm_logits_slices(int V);
+// part: 8 * B * klm_logits_parts(B, V) bytes of scratch; ids[B], best[B] the choice and its value.
+int klm_logits_parts(int B, int V);
 int klm_choose_tokens(const void* logits, int fp32, int64_t stride, int B, int V, int first, const int32_t* rows, int R,
                       const int32_t* history, int hist_len, const int32_t* prompt_lens, const int32_t* lens,
                       const float* repetition, const float* frequency, const float* presence, const int32_t* bias_ids,

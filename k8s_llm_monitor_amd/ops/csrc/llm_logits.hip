@@ -13,6 +13,7 @@
 // (whole numbers: the order of the atomic additions does not matter), then passes over the slice's logits once.
 //
 // No reference counterpart (vLLM is a README bullet in the reference, README.md:73).
+#include "klm_launch.h"
 #include "llm_common.h"
 
 using namespace klm_llm;
@@ -30,14 +31,16 @@ struct LogitArgs {
   const int* mask_rows;           // [R] mask of the row (outside 0 .. n_masks - 1: none), null: mask r for row r
   const int* rows;                // [B] rules of the row (outside 0 .. R - 1: none), null: row b
   float* out;                     // [B][V] or null
-  uint64_t* part;                 // [B][slices]
+  uint64_t* part;                 // [B][klm_logits_parts]
   int64_t* ids;                   // [B]
   float* best;                    // [B]
   int64_t stride;
   int B, V, R, hist_len, n_bias, n_masks, mask_words, first;
 };
 
-constexpr int SLICE = 4096;
+// A block takes SLICE columns, a chunk of 8 a thread. Columns are counted from the 16-byte boundary at or before the
+// row's start, so that every chunk but a row's first and last is whole aligned loads whatever the row stride is.
+constexpr int THREADS = 512, SLICE = THREADS * 8;
 
 // larger number = larger value; -0 and +0 are equal, a NaN is above everything; 0 is left for "no token"
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -75,94 +78,239 @@ __device__ __forceinline__ float apply_rules(float x, uint32_t cnt, float r, flo
   return x;
 }
 
+// One slice's 8 places of a thread as the bits that came from memory; 0 in places outside the row.
 template <bool F32>
-__global__ __launch_bounds__(256) void logits_kernel(LogitArgs a, int slices) {
-  __shared__ uint32_t cnt[SLICE];      // bit 31: in the prompt; below: times in the output
-  __shared__ uint32_t last[SLICE];     // 1 + the last bias entry of the token
-  __shared__ uint64_t red[4];
-  const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * SLICE;
-  const int n = a.V - v0 < SLICE ? a.V - v0 : SLICE;
+struct Raw {
+  uint32_t w[F32 ? 8 : 4];
+};
+template <bool F32>
+__device__ __forceinline__ void load_raw(const char* base, int v, int V, Raw<F32>& r) {
+  constexpr int ES = F32 ? 4 : 2;
+  if (v >= 0 && v + 8 <= V) {
+#pragma unroll
+    for (int k = 0; k < (F32 ? 2 : 1); ++k) {
+      const uint4 w = *reinterpret_cast<const uint4*>(base + (ptrdiff_t)v * ES + k * 16);
+      r.w[k * 4] = w.x; r.w[k * 4 + 1] = w.y; r.w[k * 4 + 2] = w.z; r.w[k * 4 + 3] = w.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < (F32 ? 8 : 4); ++k) r.w[k] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (v + e >= 0 && v + e < V) {
+        if (F32) r.w[e] = reinterpret_cast<const uint32_t*>(base)[v + e];
+        else r.w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(base)[v + e] << (16 * (e & 1));
+      }
+  }
+}
+
+// the words that hold the mask's bits of tokens t .. t + 7; t may lie before the vocabulary (places before a row's column 0) or end
+// behind it
+__device__ __forceinline__ void load_bits(const uint32_t* mask, int words, int64_t t, uint32_t& m0, uint32_t& m1) {
+  const int64_t w = t >> 5;
+  m0 = w >= 0 && w < words ? mask[w] : 0u;
+  m1 = (t & 31) > 24 && w + 1 >= 0 && w + 1 < words ? mask[w + 1] : 0u;
+}
+
+template <bool F32, bool BIAS>
+__global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs a, int slices, int per, int wide_out) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  uint32_t* cnt = lds;                 // [SLICE] bit 31: in the prompt; below: times in the output
+  uint32_t* last = lds + SLICE;        // [SLICE] 1 + the last bias entry of the token
+  __shared__ uint64_t red[THREADS / 64];
+  constexpr int ES = F32 ? 4 : 2;
+  const int tid = threadIdx.x, b = blockIdx.y, u = tid * 8;
+  const char* base = (const char*)a.logits + (size_t)b * a.stride * ES;
+  const int pad = (int)((reinterpret_cast<uintptr_t>(base) & 15) / ES);
+  const int s0 = blockIdx.x * per, s1 = s0 + per < slices ? s0 + per : slices;
+  Raw<F32> raw;
+  load_raw<F32>(base, s0 * SLICE - pad + u, a.V, raw);
   const int row = a.rows ? a.rows[b] : b;
   const bool rules = row >= 0 && row < a.R;
+
   float r = 1.f, f = 0.f, p = 0.f;
   const uint32_t* mask = nullptr;
-  const float* bias = nullptr;
+  const int *hist = nullptr, *ids = nullptr;
+  int len = 0, plen = 0;
   if (rules) {
-    const uint32_t lo = (uint32_t)a.first + v0;
-    for (int i = tid; i < n; i += 256) { cnt[i] = 0; last[i] = 0; }
-    __syncthreads();
     r = a.repetition[row];
     f = a.frequency[row];
     p = a.presence[row];
-    int len = a.lens[row];
+    len = a.lens[row];
     len = len < a.hist_len ? len : a.hist_len;
-    const int plen = a.prompt_lens[row];
-    const int* hist = a.history + (size_t)row * a.hist_len;
-    for (int i = tid; i < len; i += 256) {
-      const uint32_t t = (uint32_t)hist[i] - lo;
-      if (hist[i] >= 0 && t < (uint32_t)n) {
-        if (i >= plen) atomicAdd(&cnt[t], 1u);
-        else atomicOr(&cnt[t], 0x80000000u);
-      }
-    }
-    if (a.n_bias > 0) {
-      bias = a.bias_values + (size_t)row * a.n_bias;
-      const int* ids = a.bias_ids + (size_t)row * a.n_bias;
-      for (int i = tid; i < a.n_bias; i += 256) {
-        const uint32_t t = (uint32_t)ids[i] - lo;
-        if (ids[i] >= 0 && t < (uint32_t)n) atomicMax(&last[t], (uint32_t)i + 1);
-      }
-    }
+    plen = a.prompt_lens[row];
     if (a.mask) {
       const int m = a.mask_rows ? a.mask_rows[row] : row;
       if (m >= 0 && m < a.n_masks) mask = a.mask + (size_t)m * a.mask_words;
     }
-    __syncthreads();
+    hist = a.history + (size_t)row * a.hist_len;
+    if (BIAS) ids = a.bias_ids + (size_t)row * a.n_bias;
   }
-  uint64_t best = 0;
-  for (int i = tid; i < n; i += 256) {
-    float x = F32 ? ((const float*)a.logits)[b * a.stride + v0 + i] : bf2f(((const uint16_t*)a.logits)[b * a.stride + v0 + i]);
+  // the history's first HELD tokens a thread stay in registers for all slices; a longer one is read again from the caches
+  constexpr int HELD = 8;
+  int held[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) held[k] = tid + k * THREADS < len ? hist[tid + k * THREADS] : -1;
+  uint32_t m0 = 0, m1 = 0;             // the words of the mask that hold the 8 places' bits
+  if (mask) load_bits(mask, a.mask_words, (int64_t)a.first + s0 * SLICE - pad + u, m0, m1);
+  float top = 0.f, kept[8];            // the thread's largest value so far (valid where `kept_bits` is not 0), and the 8 values among which it is
+  uint32_t kept_bits = 0;
+  int kept_v = 0;
+  bool nan_kept = false;
+  for (int s = s0; s < s1; ++s) {
+    const int v0 = s * SLICE - pad;                                // column of the slice's first place; below 0 in a row's first slice
+    const int v = v0 + u;                                          // column of this thread's first place
+    const bool whole = v >= 0 && v + 8 <= a.V;
+    const int sh = (int)(((int64_t)a.first + v) & 31);
     if (rules) {
-      x = apply_rules(x, cnt[i], r, f, p);
-      if (bias && last[i]) x = x + bias[last[i] - 1];
+#pragma unroll
+      for (int j = 0; j < SLICE / THREADS / 4; ++j) {
+        reinterpret_cast<uint4*>(cnt)[tid + j * THREADS] = uint4{0, 0, 0, 0};
+        if (BIAS) reinterpret_cast<uint4*>(last)[tid + j * THREADS] = uint4{0, 0, 0, 0};
+      }
+      __syncthreads();
+      const uint32_t lo = (uint32_t)(a.first + v0);                // ids at or above `first` only: the difference does not wrap into the slice
+      const auto count = [&](int t, int i) {
+        const uint32_t at = (uint32_t)t - lo;
+        if (t >= a.first && at < (uint32_t)SLICE) {
+          if (i >= plen) atomicAdd(&cnt[at], 1u);
+          else atomicOr(&cnt[at], 0x80000000u);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) count(held[k], tid + k * THREADS);
+      for (int i = tid + HELD * THREADS; i < len; i += THREADS) count(hist[i], i);
+      if (BIAS) {
+        for (int i = tid; i < a.n_bias; i += THREADS) {
+          const uint32_t at = (uint32_t)ids[i] - lo;
+          if (ids[i] >= a.first && at < (uint32_t)SLICE) atomicMax(&last[at], (uint32_t)i + 1);
+        }
+      }
+      __syncthreads();
     }
-    bool allowed = true;
-    if (mask) {
-      const uint32_t t = (uint32_t)a.first + v0 + i;
-      allowed = (mask[t >> 5] >> (t & 31)) & 1;
+
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = F32 ? __uint_as_float(raw.w[e]) : __uint_as_float((e & 1) ? (raw.w[e >> 1] & 0xffff0000u) : (raw.w[e >> 1] << 16));
+    uint32_t bits = mask ? (uint32_t)((((uint64_t)m1 << 32) | m0) >> sh) & 0xffu : 0xffu;      // bit e: place e is allowed, and of the row
+    if (s + 1 < s1) {                                              // the next slice's logits and mask travel under this one's work
+      load_raw<F32>(base, v + SLICE, a.V, raw);
+      if (mask) load_bits(mask, a.mask_words, (int64_t)a.first + v + SLICE, m0, m1);
     }
-    if (a.out) a.out[(size_t)b * a.V + v0 + i] = allowed ? x : -INFINITY;
-    if (allowed) {
-      const uint64_t key = ((uint64_t)order_of(x) << 32) | (0xffffffffu - (uint32_t)(v0 + i));
-      best = key > best ? key : best;
+    if (rules) {
+      uint32_t c[8];
+      *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(cnt + u);
+      *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(cnt + u + 4);
+      if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = apply_rules(x[e], c[e], r, f, p);
+      }
+      if (BIAS) {
+        const float* bias = a.bias_values + (size_t)row * a.n_bias;
+        *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(last + u);
+        *reinterpret_cast<uint4*>(c + 4) = *reinterpret_cast<const uint4*>(last + u + 4);
+        if ((c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) != 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c[e]) x[e] = x[e] + bias[c[e] - 1];
+        }
+      }
+      if (s + 1 < s1) __syncthreads();                             // the counts are cleared for the next slice
+    }
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits &= v + e >= 0 && v + e < a.V ? 0xffu : ~(1u << e);
+    }
+    if (mask || !whole) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (bits >> e) & 1 ? x[e] : -INFINITY;
+    }
+    if (a.out) {
+      float* dst = a.out + (size_t)b * a.V + v;
+      if (wide_out && whole) {
+        *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (v + e >= 0 && v + e < a.V) dst[e] = x[e];
+      }
+    }
+    // the largest value by a plain maximum; its column is looked for at the end, by the threads that hold the block's largest
+    float m = x[0];
+    bool nan = __builtin_isunordered(x[0], x[1]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      m = fmaxf(m, x[e]);
+      if (e & 1) nan = nan || __builtin_isunordered(x[e], x[e - 1]);
+    }
+    // an equal value of a later slice has a higher column; the first slice with a NaN is kept for good
+    if (bits && !nan_kept && (nan || !kept_bits || m > top)) {
+      top = m;
+      kept_bits = bits;
+      kept_v = v;
+      nan_kept = nan;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kept[e] = x[e];
     }
   }
-  best = wave_max(best);
-  if ((tid & 63) == 0) red[tid >> 6] = best;
+  const uint32_t mine = nan_kept ? 0xffffffffu : kept_bits ? order_of(top) : 0u;
+  uint32_t most = mine;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(most, o);
+    most = other > most ? other : most;
+  }
+  uint32_t at = 0xffffffffu;
+  if (mine == most && most != 0) {
+#pragma unroll
+    for (int e = 7; e >= 0; --e) at = (kept_bits >> e) & 1 && order_of(kept[e]) == most ? (uint32_t)(kept_v + e) : at;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(at, o);
+    at = other < at ? other : at;
+  }
+  if ((tid & 63) == 0) red[tid >> 6] = most ? ((uint64_t)most << 32) | (0xffffffffu - at) : 0;
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < 4; ++i) best = red[i] > best ? red[i] : best;
-    if (slices == 1) write_choice(a, b, best);
-    else a.part[(size_t)b * slices + blockIdx.x] = best;
+    uint64_t best = red[0];
+    for (int i = 1; i < THREADS / 64; ++i) best = red[i] > best ? red[i] : best;
+    if (gridDim.x == 1) write_choice(a, b, best);
+    else a.part[(size_t)b * gridDim.x + blockIdx.x] = best;
   }
 }
 
-__global__ __launch_bounds__(64) void choose_kernel(LogitArgs a, int slices) {
+__global__ __launch_bounds__(64) void choose_kernel(LogitArgs a, int parts) {
   const int b = blockIdx.x;
   uint64_t best = 0;
-  for (int i = threadIdx.x; i < slices; i += 64) {
-    const uint64_t k = a.part[(size_t)b * slices + i];
+  for (int i = threadIdx.x; i < parts; i += 64) {
+    const uint64_t k = a.part[(size_t)b * parts + i];
     best = k > best ? k : best;
   }
   best = wave_max(best);
   if (threadIdx.x == 0) write_choice(a, b, best);
 }
 
+int slices_of(int V) { return (int)(((int64_t)V + 7 + SLICE - 1) / SLICE); }     // a row may start up to 7 places into its first slice
+// Slices that one block walks: as few as let all blocks be on the chip at once (4 per CU). A block's chain of dependent loads
+// (the row's lengths, its history, the mask) is longer than the work of a slice: 96 x 128256 in rounds of one slice 18.9 us.
+int slices_per_block(int B, int V) {
+  const int slices = slices_of(V);
+  int per = 1;
+  while (per < 8 && (int64_t)((slices + per - 1) / per) * B > 1024) ++per;
+  return per;
+}
+
 }  // namespace
 
 extern "C" {
 
-int klm_logits_slices(int V) { return (V + SLICE - 1) / SLICE; }
+int klm_logits_parts(int B, int V) {
+  const int per = slices_per_block(B, V);
+  return (slices_of(V) + per - 1) / per;
+}
 
 int klm_choose_tokens(const void* logits, int fp32, int64_t stride, int B, int V, int first, const int32_t* rows, int R,
                       const int32_t* history, int hist_len, const int32_t* prompt_lens, const int32_t* lens,
@@ -179,12 +327,24 @@ int klm_choose_tokens(const void* logits, int fp32, int64_t stride, int B, int V
   LogitArgs a{logits, history, prompt_lens, lens, repetition, frequency, presence, bias_ids, bias_values,
               n_masks > 0 ? (const uint32_t*)mask : nullptr, mask_rows, rows, out, (uint64_t*)part, ids, best, stride,
               B, V, R, hist_len, n_bias, n_masks, mask_words, first};
-  const int slices = klm_logits_slices(V);
+  const int slices = slices_of(V), per = slices_per_block(B, V), parts = klm_logits_parts(B, V);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (fp32) hipLaunchKernelGGL(logits_kernel<true>, dim3(slices, B), dim3(256), 0, s, a, slices);
-  else hipLaunchKernelGGL(logits_kernel<false>, dim3(slices, B), dim3(256), 0, s, a, slices);
+  // 16-byte stores where every chunk starts on such a boundary of `out`: columns there and in `logits` are off alike
+  const int pad = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / (fp32 ? 4 : 2));
+  const int wide_out = out && pad % 4 == 0 && (B == 1 || (V % 4 == 0 && stride % (fp32 ? 4 : 8) == 0)) && aligned16(out);
+  const dim3 grid(parts, B);
+  const size_t one = SLICE * 4;
+  if (n_bias > 0 && R > 0) {
+    if ((fp32 ? klm_ensure_dyn_lds<logits_kernel<true, true>>(2 * one) : klm_ensure_dyn_lds<logits_kernel<false, true>>(2 * one)) != KLM_OK)
+      return KLM_ERR_HIP;
+    if (fp32) hipLaunchKernelGGL((logits_kernel<true, true>), grid, dim3(THREADS), 2 * one, s, a, slices, per, wide_out);
+    else hipLaunchKernelGGL((logits_kernel<false, true>), grid, dim3(THREADS), 2 * one, s, a, slices, per, wide_out);
+  } else {
+    if (fp32) hipLaunchKernelGGL((logits_kernel<true, false>), grid, dim3(THREADS), one, s, a, slices, per, wide_out);
+    else hipLaunchKernelGGL((logits_kernel<false, false>), grid, dim3(THREADS), one, s, a, slices, per, wide_out);
+  }
   if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
-  if (slices > 1) hipLaunchKernelGGL(choose_kernel, dim3(B), dim3(64), 0, s, a, slices);
+  if (parts > 1) hipLaunchKernelGGL(choose_kernel, dim3(B), dim3(64), 0, s, a, parts);
   return launch_status();
 }
 

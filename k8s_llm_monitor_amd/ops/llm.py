@@ -64,9 +64,9 @@ def _lib():
         lib.klm_window_attn_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, vp]
         lib.klm_window_attn_prefill.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, i, vp]
         lib.klm_copy_pages.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp]
-        lib.klm_logits_slices.argtypes = [i]
+        lib.klm_logits_parts.argtypes = [i, i]
         lib.klm_choose_tokens.argtypes = [vp, i, i64, i, i, i, vp, i, vp, i, vp, vp, vp, vp, vp, vp, vp, i, vp, i, i, vp, vp, vp, vp, vp, vp]
-        for n in ("klm_window_attn_decode", "klm_window_attn_prefill", "klm_copy_pages", "klm_logits_slices", "klm_choose_tokens"):
+        for n in ("klm_window_attn_decode", "klm_window_attn_prefill", "klm_copy_pages", "klm_logits_parts", "klm_choose_tokens"):
             getattr(lib, n).restype = i
         for n in ("klm_rmsnorm", "klm_silu_mul", "klm_rope_cache", "klm_paged_attn_decode", "klm_paged_attn_prefill",
                   "klm_skinny_linear"):
@@ -891,7 +891,7 @@ def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, firs
     if B == 0:
         return ids, best
     lib = _lib()
-    part = torch.empty((B, lib.klm_logits_slices(V)), dtype=torch.int64, device=logits.device)
+    part = torch.empty((B, lib.klm_logits_parts(B, V)), dtype=torch.int64, device=logits.device)
     r = rules
 
     def ptr(t: Optional[torch.Tensor]):
