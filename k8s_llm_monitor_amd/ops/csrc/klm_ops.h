@@ -184,33 +184,55 @@ int klm_rope_cache_from_partials(const float* part, int ksplit, void* qkv, const
 int klm_mid_epilogue(const float* part, int ksplit, int M, int N, int kind, void* out, void* residual, float eps, void* stream);
 
 // Attention with a sliding window and sinks over the paged cache (llm_window.hip): the token at position p sees key j when
-// j <= p and (j > p - window or j < sinks) and the page table has a page of the cache for it (0 <= id < num_blocks). Decode: q
-// row b stands at position ctx_lens[b] - 1; part_o [B][n_q][num_splits][128] and part_ml [B][n_q][num_splits][2] (fp32) are
-// scratch for num_splits > 1. Prefill: seq_info[n_seqs][3] = {q_start, q_len, ctx_len}, rows of no sequence are not written;
-// q_tiles: 32-row query tiles per wave (1 or 2).
-int klm_window_attn_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                           const int32_t* ctx_lens, void* out, float* part_o, float* part_ml, int B, int q_stride, int n_q,
-                           int n_kv, int max_blocks, int num_blocks, int window, int sinks, int num_splits, float scale,
-                           int kv_fp8, void* stream);
-int klm_window_attn_prefill(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                            const int32_t* seq_info, void* out, int T, int n_seqs, int q_stride, int n_q, int n_kv,
-                            int max_blocks, int num_blocks, int window, int sinks, float scale, int q_tiles, int kv_fp8, void* stream);
+// j <= p and (j > p - window or j < sinks) and the page table has a page of the cache for it (0 <= id < pages). Decode: `lens` is
+// ctx_lens[n_seqs], q row b stands at position ctx_lens[b] - 1. Prefill: `lens` is seq_info[n_seqs][3] = {q_start, q_len,
+// ctx_len}; rows of no sequence are not written. splits > 1: part_o [rows][n_q][splits][128] and part_ml
+// [rows][n_q][splits][2] (fp32) are scratch. One struct instead of twenty arguments: a call from Python costs a microsecond less.
+typedef struct klm_window_args {
+  const void *q, *k_cache, *v_cache;
+  const int32_t *tables, *lens;      // tables[n_seqs][width]
+  void* out;                         // [rows][n_q][128]
+  float *part_o, *part_ml;
+  void* stream;
+  int n_seqs, rows, q_stride, n_q, n_kv, width, pages, window, sinks, splits, kv_fp8;
+  float scale;
+} klm_window_args;
+int klm_window_attn_decode(const klm_window_args* args);
+int klm_window_attn_prefill(const klm_window_args* args);
 
 // Pages of a cache [layers][blocks][n_kv][2048 elements], K and V (llm_pages.hip): page pairs[2i] of the source goes to page
 // pairs[2i + 1] of the destination in every layer (a source < 0 clears). `pairs` is host memory, read before the call
 // returns; source and destination may be one cache when no page that is written is read by another pair.
-int klm_copy_pages(const void* k_src, const void* v_src, void* k_dst, void* v_dst, const int32_t* pairs, int n, int layers,
-                   int src_blocks, int dst_blocks, int n_kv, int elem_size, void* stream);
+typedef struct klm_pages_args {
+  const void *k_src, *v_src;
+  void *k_dst, *v_dst;
+  const int32_t* pairs;              // [n][2]
+  void* stream;
+  int n, layers, src_blocks, dst_blocks, n_kv, elem_size;
+} klm_pages_args;
+int klm_copy_pages(const klm_pages_args* args);
 
 // Rules on logits and the greedy choice (llm_logits.hip): logits[B][V] bf16 or fp32, `first` the token id of column 0, R sets
 // of rules, rows[B] the set of each row (null: its own number; outside 0 .. R - 1: none). out [B][V] fp32 or null;
 // part: 8 * B * klm_logits_parts(B, V) bytes of scratch; ids[B], best[B] the choice and its value.
+typedef struct klm_logits_args {
+  const void* logits;
+  const int32_t *rows, *history, *prompt_lens, *lens;                // history [R][hist_len]
+  const float *repetition, *frequency, *presence;                    // [R]
+  const int32_t* bias_ids;                                           // [R][n_bias]
+  const float* bias_values;
+  const void* mask;                                                  // [n_masks][mask_words]
+  const int32_t* mask_rows;                                          // [R] or null: mask r for set r
+  float* out;
+  void* part;
+  int64_t* ids;
+  float* best;
+  void* stream;
+  int64_t stride;
+  int fp32, B, V, first, R, hist_len, n_bias, n_masks, mask_words, pad;
+} klm_logits_args;
 int klm_logits_parts(int B, int V);
-int klm_choose_tokens(const void* logits, int fp32, int64_t stride, int B, int V, int first, const int32_t* rows, int R,
-                      const int32_t* history, int hist_len, const int32_t* prompt_lens, const int32_t* lens,
-                      const float* repetition, const float* frequency, const float* presence, const int32_t* bias_ids,
-                      const float* bias_values, int n_bias, const void* mask, int n_masks, int mask_words,
-                      const int32_t* mask_rows, float* out, void* part, int64_t* ids, float* best, void* stream);
+int klm_choose_tokens(const klm_logits_args* args);
 
 const char* klm_version(void);
 const char* klm_src_hash(void);   /* hash of the sources this library was built from (build.py), "unhashed" otherwise */

@@ -312,29 +312,28 @@ int klm_logits_parts(int B, int V) {
   return (slices_of(V) + per - 1) / per;
 }
 
-int klm_choose_tokens(const void* logits, int fp32, int64_t stride, int B, int V, int first, const int32_t* rows, int R,
-                      const int32_t* history, int hist_len, const int32_t* prompt_lens, const int32_t* lens,
-                      const float* repetition, const float* frequency, const float* presence, const int32_t* bias_ids,
-                      const float* bias_values, int n_bias, const void* mask, int n_masks, int mask_words,
-                      const int32_t* mask_rows, float* out, void* part, int64_t* ids, float* best, void* stream) {
-  if (B <= 0 || B > 65535 || V <= 0 || stride < V || first < 0 || (int64_t)first + V > INT32_MAX || R < 0 || hist_len < 0 || n_bias < 0 ||
-      n_masks < 0)
+int klm_choose_tokens(const klm_logits_args* c) {
+  if (!c) return KLM_ERR_ARG;
+  const int B = c->B, V = c->V, fp32 = c->fp32;
+  if (B <= 0 || B > 65535 || V <= 0 || c->stride < V || c->first < 0 || (int64_t)c->first + V > INT32_MAX || c->R < 0 || c->hist_len < 0 ||
+      c->n_bias < 0 || c->n_masks < 0)
     return KLM_ERR_SHAPE;
-  if (!logits || !ids || !best || !part) return KLM_ERR_ARG;
-  if (R > 0 && (!prompt_lens || !lens || !repetition || !frequency || !presence || (hist_len > 0 && !history) ||
-                (n_bias > 0 && (!bias_ids || !bias_values)) || (n_masks > 0 && (!mask || (int64_t)mask_words * 32 < (int64_t)first + V))))
+  if (!c->logits || !c->ids || !c->best || !c->part) return KLM_ERR_ARG;
+  if (c->R > 0 && (!c->prompt_lens || !c->lens || !c->repetition || !c->frequency || !c->presence || (c->hist_len > 0 && !c->history) ||
+                   (c->n_bias > 0 && (!c->bias_ids || !c->bias_values)) ||
+                   (c->n_masks > 0 && (!c->mask || (int64_t)c->mask_words * 32 < (int64_t)c->first + V))))
     return KLM_ERR_ARG;
-  LogitArgs a{logits, history, prompt_lens, lens, repetition, frequency, presence, bias_ids, bias_values,
-              n_masks > 0 ? (const uint32_t*)mask : nullptr, mask_rows, rows, out, (uint64_t*)part, ids, best, stride,
-              B, V, R, hist_len, n_bias, n_masks, mask_words, first};
+  const LogitArgs a{c->logits, c->history, c->prompt_lens, c->lens, c->repetition, c->frequency, c->presence, c->bias_ids, c->bias_values,
+                    c->n_masks > 0 ? (const uint32_t*)c->mask : nullptr, c->mask_rows, c->rows, c->out, (uint64_t*)c->part, c->ids, c->best,
+                    c->stride, B, V, c->R, c->hist_len, c->n_bias, c->n_masks, c->mask_words, c->first};
   const int slices = slices_of(V), per = slices_per_block(B, V), parts = klm_logits_parts(B, V);
-  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipStream_t s = static_cast<hipStream_t>(c->stream);
   // 16-byte stores where every chunk starts on such a boundary of `out`: columns there and in `logits` are off alike
-  const int pad = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / (fp32 ? 4 : 2));
-  const int wide_out = out && pad % 4 == 0 && (B == 1 || (V % 4 == 0 && stride % (fp32 ? 4 : 8) == 0)) && aligned16(out);
+  const int pad = (int)((reinterpret_cast<uintptr_t>(c->logits) & 15) / (fp32 ? 4 : 2));
+  const int wide_out = a.out && pad % 4 == 0 && (B == 1 || (V % 4 == 0 && a.stride % (fp32 ? 4 : 8) == 0)) && aligned16(a.out);
   const dim3 grid(parts, B);
   const size_t one = SLICE * 4;
-  if (n_bias > 0 && R > 0) {
+  if (a.n_bias > 0 && a.R > 0) {
     if ((fp32 ? klm_ensure_dyn_lds<logits_kernel<true, true>>(2 * one) : klm_ensure_dyn_lds<logits_kernel<false, true>>(2 * one)) != KLM_OK)
       return KLM_ERR_HIP;
     if (fp32) hipLaunchKernelGGL((logits_kernel<true, true>), grid, dim3(THREADS), 2 * one, s, a, slices, per, wide_out);

@@ -49,21 +49,23 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(PageArgs a, PagePairs p
 
 extern "C" {
 
-int klm_copy_pages(const void* k_src, const void* v_src, void* k_dst, void* v_dst, const int32_t* pairs, int n, int layers,
-                   int src_blocks, int dst_blocks, int n_kv, int elem_size, void* stream) {
-  if (n < 0 || layers <= 0 || layers > 65535 || src_blocks <= 0 || dst_blocks <= 0 || n_kv <= 0) return KLM_ERR_SHAPE;
-  if ((elem_size != 1 && elem_size != 2) || (n > 0 && !pairs) || !k_src || !v_src || !k_dst || !v_dst) return KLM_ERR_ARG;
-  if (!aligned16(k_src) || !aligned16(v_src) || !aligned16(k_dst) || !aligned16(v_dst)) return KLM_ERR_ALIGN;
+int klm_copy_pages(const klm_pages_args* c) {
+  if (!c) return KLM_ERR_ARG;
+  const int n = c->n;
+  const int32_t* pairs = c->pairs;
+  if (n < 0 || c->layers <= 0 || c->layers > 65535 || c->src_blocks <= 0 || c->dst_blocks <= 0 || c->n_kv <= 0) return KLM_ERR_SHAPE;
+  if ((c->elem_size != 1 && c->elem_size != 2) || (n > 0 && !pairs) || !c->k_src || !c->v_src || !c->k_dst || !c->v_dst) return KLM_ERR_ARG;
+  if (!aligned16(c->k_src) || !aligned16(c->v_src) || !aligned16(c->k_dst) || !aligned16(c->v_dst)) return KLM_ERR_ALIGN;
   for (int i = 0; i < n; ++i)
-    if (pairs[2 * i] >= src_blocks || pairs[2 * i + 1] < 0 || pairs[2 * i + 1] >= dst_blocks) return KLM_ERR_ARG;
+    if (pairs[2 * i] >= c->src_blocks || pairs[2 * i + 1] < 0 || pairs[2 * i + 1] >= c->dst_blocks) return KLM_ERR_ARG;
   PageArgs a;
-  a.ks = (const char*)k_src;
-  a.vs = (const char*)v_src;
-  a.kd = (char*)k_dst;
-  a.vd = (char*)v_dst;
-  a.slab = (size_t)n_kv * BLK_ELEMS * elem_size;
-  a.src_layer = a.slab * src_blocks;
-  a.dst_layer = a.slab * dst_blocks;
+  a.ks = (const char*)c->k_src;
+  a.vs = (const char*)c->v_src;
+  a.kd = (char*)c->k_dst;
+  a.vd = (char*)c->v_dst;
+  a.slab = (size_t)c->n_kv * BLK_ELEMS * c->elem_size;
+  a.src_layer = a.slab * c->src_blocks;
+  a.dst_layer = a.slab * c->dst_blocks;
   const size_t chunks = (a.slab + PER_BLOCK - 1) / PER_BLOCK;
   if (chunks > 65535) return KLM_ERR_SHAPE;
   a.chunks = (int)chunks;
@@ -74,7 +76,7 @@ int klm_copy_pages(const void* k_src, const void* v_src, void* k_dst, void* v_ds
       p.src[i] = i < m ? pairs[2 * (at + i)] : -1;
       p.dst[i] = i < m ? pairs[2 * (at + i) + 1] : 0;
     }
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(m * a.chunks), layers, 2), dim3(256), 0, static_cast<hipStream_t>(stream), a, p);
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(m * a.chunks), c->layers, 2), dim3(256), 0, static_cast<hipStream_t>(c->stream), a, p);
     if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
   }
   return KLM_OK;

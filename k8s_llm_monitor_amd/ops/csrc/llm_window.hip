@@ -569,52 +569,46 @@ int check_args(const WinArgs& a) {
   return KLM_OK;
 }
 
+WinArgs device_args(const klm_window_args* c) {
+  return WinArgs{(const uint16_t*)c->q, c->k_cache, c->v_cache, c->tables, c->lens, (uint16_t*)c->out, c->part_o, c->part_ml,
+                 c->n_seqs, c->rows, c->q_stride, c->n_q, c->n_kv, c->n_kv > 0 ? c->n_q / c->n_kv : 0, c->width, c->pages,
+                 c->window, c->sinks, c->splits, c->scale * 1.4426950408889634f};
+}
+
 }  // namespace
 
 extern "C" {
 
-int klm_window_attn_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                           const int32_t* ctx_lens, void* out, float* part_o, float* part_ml, int B, int q_stride, int n_q,
-                           int n_kv, int max_blocks, int num_blocks, int window, int sinks, int num_splits, float scale,
-                           int kv_fp8, void* stream) {
-  WinArgs a{(const uint16_t*)q, k_cache, v_cache, block_tables, ctx_lens, (uint16_t*)out, part_o, part_ml, B, B,
-            q_stride, n_q, n_kv, n_kv > 0 ? n_q / n_kv : 0, max_blocks, num_blocks, window, sinks, num_splits, scale * 1.4426950408889634f};
+int klm_window_attn_decode(const klm_window_args* c) {
+  if (!c) return KLM_ERR_ARG;
+  const WinArgs a = device_args(c);
   const int rc = check_args(a);
   if (rc != KLM_OK) return rc;
+  if (a.n_seqs != a.rows) return KLM_ERR_SHAPE;
   const int head_tiles = (a.G + 15) / 16;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(n_kv * head_tiles, B, num_splits);
-  if (kv_fp8) hipLaunchKernelGGL(window_decode_kernel<true>, grid, dim3(256), 0, s, a, head_tiles);
+  hipStream_t s = static_cast<hipStream_t>(c->stream);
+  const dim3 grid(a.n_kv * head_tiles, a.rows, a.splits);
+  if (c->kv_fp8) hipLaunchKernelGGL(window_decode_kernel<true>, grid, dim3(256), 0, s, a, head_tiles);
   else hipLaunchKernelGGL(window_decode_kernel<false>, grid, dim3(256), 0, s, a, head_tiles);
   if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
-  if (num_splits > 1) {
-    const size_t heads = (size_t)B * n_q;
+  if (a.splits > 1) {
+    const size_t heads = (size_t)a.rows * a.n_q;
     hipLaunchKernelGGL(window_join_kernel, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a, heads);
   }
   return launch_status();
 }
 
-int klm_window_attn_prefill(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                            const int32_t* seq_info, void* out, int T, int n_seqs, int q_stride, int n_q, int n_kv,
-                            int max_blocks, int num_blocks, int window, int sinks, float scale, int q_tiles, int kv_fp8, void* stream) {
-  WinArgs a{(const uint16_t*)q, k_cache, v_cache, block_tables, seq_info, (uint16_t*)out, nullptr, nullptr, n_seqs, T,
-            q_stride, n_q, n_kv, n_kv > 0 ? n_q / n_kv : 0, max_blocks, num_blocks, window, sinks, 1, scale * 1.4426950408889634f};
+int klm_window_attn_prefill(const klm_window_args* c) {
+  if (!c) return KLM_ERR_ARG;
+  const WinArgs a = device_args(c);
   const int rc = check_args(a);
   if (rc != KLM_OK) return rc;
-  if (q_tiles != 1 && q_tiles != 2) return KLM_ERR_VARIANT;
-  const int64_t tiles = ((int64_t)T * a.G + 128 * q_tiles - 1) / (128 * q_tiles) + n_seqs;   // every sequence may end in a partial tile
+  const int64_t tiles = ((int64_t)a.rows * a.G + 255) / 256 + a.n_seqs;       // every sequence may end in a partial tile
   if (tiles > 65535) return KLM_ERR_SHAPE;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(n_kv, (unsigned)tiles, 1);
-#define KLM_LAUNCH(QT, F8) hipLaunchKernelGGL((window_prefill_kernel<QT, F8>), grid, dim3(256), 2 * STEP_BYTES, s, a)
-  if (q_tiles == 1) {
-    if (kv_fp8) KLM_LAUNCH(1, true);
-    else KLM_LAUNCH(1, false);
-  } else {
-    if (kv_fp8) KLM_LAUNCH(2, true);
-    else KLM_LAUNCH(2, false);
-  }
-#undef KLM_LAUNCH
+  hipStream_t s = static_cast<hipStream_t>(c->stream);
+  const dim3 grid(a.n_kv, (unsigned)tiles, 1);
+  if (c->kv_fp8) hipLaunchKernelGGL((window_prefill_kernel<2, true>), grid, dim3(256), 2 * STEP_BYTES, s, a);
+  else hipLaunchKernelGGL((window_prefill_kernel<2, false>), grid, dim3(256), 2 * STEP_BYTES, s, a);
   return launch_status();
 }
 

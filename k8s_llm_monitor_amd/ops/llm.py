@@ -10,16 +10,15 @@ No reference counterpart (vLLM is a README bullet in the reference, README.md:73
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-from dataclasses import dataclass
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from . import KlmOpsError, _check, _on_device, load
-from . import _stream_of as _stream
+from . import _stream_of
 from . import ref
 
 HEAD_DIM = ref.HEAD_DIM
@@ -27,6 +26,12 @@ BLOCK = ref.BLOCK
 rope_table = ref.rope_table
 
 _bound = False
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device, as a number (2 us less than through a torch.cuda.Stream object)."""
+    return _raw_stream(t.device.index) if _raw_stream is not None else _stream_of(t)
 
 
 def _lib():
@@ -61,11 +66,10 @@ def _lib():
         for n in ("klm_mid_linear_plan", "klm_mid_linear", "klm_mid_linear_w8", "klm_mid_epilogue", "klm_rope_cache_from_partials",
                   "klm_mid_linear_swiglu"):
             getattr(lib, n).restype = i
-        lib.klm_window_attn_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, vp]
-        lib.klm_window_attn_prefill.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, i, vp]
-        lib.klm_copy_pages.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp]
+        # these take a struct of their arguments, packed by `struct`: ctypes converts one pointer instead of twenty values
+        lib.klm_window_attn_decode.argtypes = lib.klm_window_attn_prefill.argtypes = lib.klm_choose_tokens.argtypes = [ctypes.c_char_p]
+        lib.klm_copy_pages.argtypes = [ctypes.c_char_p]
         lib.klm_logits_parts.argtypes = [i, i]
-        lib.klm_choose_tokens.argtypes = [vp, i, i64, i, i, i, vp, i, vp, i, vp, vp, vp, vp, vp, vp, vp, i, vp, i, i, vp, vp, vp, vp, vp, vp]
         for n in ("klm_window_attn_decode", "klm_window_attn_prefill", "klm_copy_pages", "klm_logits_parts", "klm_choose_tokens"):
             getattr(lib, n).restype = i
         for n in ("klm_rmsnorm", "klm_silu_mul", "klm_rope_cache", "klm_paged_attn_decode", "klm_paged_attn_prefill",
@@ -605,41 +609,40 @@ def paged_attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
 
 # ------------------------------------------------------------------ sliding window and sinks
-_HERE = contextlib.nullcontext()
-
-
-def _launch_on(t: torch.Tensor):
-    """The device that a launch for `t` has to be made on, where it is not the current one."""
-    return _HERE if t.device.index == torch.cuda.current_device() else _on_device(t)
-
-
-def _same_device(what: str, t: torch.Tensor, *others) -> None:
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise KlmOpsError(f"{what}: tensors on {t.device} and {o.device}")
-
-
 _FAR = 1 << 30          # a window or sinks beyond any context; keeps the kernels' 32-bit positions from running over
+_WINDOW_ARGS = struct.Struct("9P11if")          # klm_window_args
 
 
-def _check_window(what: str, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out) -> Tuple[int, int, int]:
-    """-> blocks of the cache, window, sinks."""
-    n_kv = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    nb = _check_caches(k_cache, v_cache, n_kv)
-    if nb < 1 or n_kv < 1 or n_q < 1 or n_q % n_kv:
-        raise KlmOpsError(f"{what}: {n_q} query heads, cache {tuple(k_cache.shape)}")
+def _call(fn, args: bytes, t: torch.Tensor) -> int:
+    """A launcher on the device of `t`, whichever is current."""
+    if t.device.index == torch.cuda.current_device():
+        return fn(args)
+    with _on_device(t):
+        return fn(args)
+
+
+def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q, window, sinks, out) -> None:
+    ks, dev = k_cache.shape, q.device
+    if len(ks) != 4 or len(v_cache.shape) != 4:
+        raise KlmOpsError(f"{what}: cache shapes K {tuple(ks)} V {tuple(v_cache.shape)}")
+    _check_caches(k_cache, v_cache, ks[1])
+    if ks[0] < 1 or ks[1] < 1 or n_q < 1 or n_q % ks[1]:
+        raise KlmOpsError(f"{what}: {n_q} query heads, cache {tuple(ks)}")
     if q.dim() != 2 or q.shape[1] < n_q * HEAD_DIM or q.stride(1) != 1 or (q.shape[0] > 1 and q.stride(0) < n_q * HEAD_DIM):
         raise KlmOpsError(f"{what}: q {tuple(q.shape)} strides {q.stride()} for {n_q} heads")
     if block_tables.dim() != 2 or block_tables.shape[1] < 1:
         raise KlmOpsError(f"{what}: block_tables {tuple(block_tables.shape)}")
-    if int(window) < 1 or int(sinks) < 0:
+    if window < 1 or sinks < 0:
         raise KlmOpsError(f"{what}: window {window} (at least 1: the token itself), sinks {sinks}")
-    if not 0.0 < float(scale) < float("inf"):
+    if not 0.0 < scale < float("inf"):
         raise KlmOpsError(f"{what}: scale {scale}")
-    if out is not None and (tuple(out.shape) != (q.shape[0], n_q * HEAD_DIM) or out.dtype != q.dtype or not out.is_contiguous()):
-        raise KlmOpsError(f"{what}: out {tuple(out.shape)} {out.dtype}")
-    _same_device(what, q, k_cache, v_cache, block_tables, out)
-    return nb, min(int(window), _FAR), min(int(sinks), _FAR)
+    if out is not None and (tuple(out.shape) != (q.shape[0], n_q * HEAD_DIM) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev):
+        raise KlmOpsError(f"{what}: out {tuple(out.shape)} {out.dtype} {out.device}")
+    if k_cache.device != dev or v_cache.device != dev or block_tables.device != dev or lens.device != dev:
+        raise KlmOpsError(f"{what}: tensors on different devices")
+    if q.is_cuda:
+        _bf16(q)
+        _i32(block_tables, lens)
 
 
 def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -653,38 +656,41 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     Pages between the sinks and the window are not looked at: their table entries may hold anything. An entry outside the
     cache (-1) is no page and its tokens are not seen, nor are tokens beyond the table. A sequence that sees nothing (length
     0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `num_splits` 0: chosen from the shapes.
-    `workspace`: the splits' scratch, for calls that must not share it with the allocator; one per stream."""
+    `workspace`: the splits' scratch, for calls that must not take it from the allocator; calls that may run at the same time
+    need one each."""
     what = "paged_attn_decode_window"
-    nb, window, sinks = _check_window(what, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out)
+    _check_window(what, q, k_cache, v_cache, block_tables, ctx_lens, scale, n_q, window, sinks, out)
     B, width = block_tables.shape
-    n_kv = k_cache.shape[1]
+    nb, n_kv = k_cache.shape[:2]
     if q.shape[0] != B or ctx_lens.shape != (B,):
         raise KlmOpsError(f"{what}: q {tuple(q.shape)}, ctx_lens {tuple(ctx_lens.shape)} for {B} table rows")
-    if not 0 <= int(num_splits) <= 256:
+    if not 0 <= num_splits <= 256:
         raise KlmOpsError(f"{what}: num_splits {num_splits}")
-    _same_device(what, q, ctx_lens)
     if not q.is_cuda:
         o = ref.window_attn_decode(q[:, : n_q * HEAD_DIM], k_cache, v_cache, block_tables, ctx_lens, scale, window, sinks)
         return o if out is None else out.copy_(o)
-    _bf16(q)
-    _i32(block_tables, ctx_lens)
     if out is None:
-        out = torch.empty((B, n_q * HEAD_DIM), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, n_q * HEAD_DIM))
     if B == 0:
         return out
-    splits = int(num_splits) or pick_splits(B, n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
-    part_o = part_ml = None
+    window, sinks = min(window, _FAR), min(sinks, _FAR)
+    splits = num_splits or pick_splits(B, n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
+    part_o = part_ml = 0
     if splits > 1:
         if workspace is None:
-            workspace = DecodeWorkspace(B, n_q, splits, q.device)
-        if workspace.max_batch < B or workspace.n_q != n_q or workspace.max_splits < splits or workspace.tmp_o.device != q.device:
-            raise KlmOpsError(f"{what}: workspace too small")
-        part_o, part_ml = workspace.tmp_o.data_ptr(), workspace.tmp_ml.data_ptr()
-    with _launch_on(q):
-        rc = _lib().klm_window_attn_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-                                           ctx_lens.data_ptr(), out.data_ptr(), part_o, part_ml, B, q.stride(0), n_q, n_kv, width, nb,
-                                           window, sinks, splits, float(scale), _kv8(k_cache), _stream(q))
-    _check(rc, f"klm_window_attn_decode(B={B},window={window},sinks={sinks},splits={splits})")
+            scratch = torch.empty(B * n_q * splits * (HEAD_DIM + 2), dtype=torch.float32, device=q.device)
+            part_o = scratch.data_ptr()
+            part_ml = part_o + B * n_q * splits * HEAD_DIM * 4
+        else:
+            if workspace.max_batch < B or workspace.n_q != n_q or workspace.max_splits < splits or workspace.tmp_o.device != q.device:
+                raise KlmOpsError(f"{what}: workspace too small")
+            part_o, part_ml = workspace.tmp_o.data_ptr(), workspace.tmp_ml.data_ptr()
+    rc = _call(_lib().klm_window_attn_decode,
+               _WINDOW_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), ctx_lens.data_ptr(),
+                                 out.data_ptr(), part_o, part_ml, _stream(q), B, B, q.stride(0) if B > 1 else n_q * HEAD_DIM, n_q, n_kv,
+                                 width, nb, window, sinks, splits, _kv8(k_cache), scale), q)
+    if rc:
+        _check(rc, f"klm_window_attn_decode(B={B},window={window},sinks={sinks},splits={splits})")
     return out
 
 
@@ -698,30 +704,31 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     captured call may be replayed with others. The sequences' rows must not overlap. Rows of no sequence (padding, or one
     with q_len <= 0 or ctx_len < q_len) stay as they are in a given `out` and are zero otherwise."""
     what = "paged_attn_prefill_window"
-    nb, window, sinks = _check_window(what, q, k_cache, v_cache, block_tables, scale, n_q, window, sinks, out)
+    _check_window(what, q, k_cache, v_cache, block_tables, seq_info, scale, n_q, window, sinks, out)
     S, width = block_tables.shape
-    n_kv = k_cache.shape[1]
+    nb, n_kv = k_cache.shape[:2]
     T = q.shape[0]
     if tuple(seq_info.shape) != (S, 3):
         raise KlmOpsError(f"{what}: seq_info {tuple(seq_info.shape)} for {S} table rows")
-    _same_device(what, q, seq_info)
     if not q.is_cuda:
         return ref.window_attn_prefill(q[:, : n_q * HEAD_DIM], k_cache, v_cache, block_tables, seq_info, scale, window, sinks, out)
-    _bf16(q)
-    _i32(block_tables, seq_info)
     if out is None:
-        out = torch.zeros((T, n_q * HEAD_DIM), dtype=q.dtype, device=q.device)
+        out = q.new_zeros((T, n_q * HEAD_DIM))
     if T == 0 or S == 0:
         return out
-    with _launch_on(q):
-        rc = _lib().klm_window_attn_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-                                            seq_info.data_ptr(), out.data_ptr(), T, S, q.stride(0), n_q, n_kv, width, nb,
-                                            window, sinks, float(scale), 2, _kv8(k_cache), _stream(q))
-    _check(rc, f"klm_window_attn_prefill(T={T},S={S},window={window},sinks={sinks})")
+    rc = _call(_lib().klm_window_attn_prefill,
+               _WINDOW_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_info.data_ptr(),
+                                 out.data_ptr(), 0, 0, _stream(q), S, T, q.stride(0) if T > 1 else n_q * HEAD_DIM, n_q, n_kv, width, nb,
+                                 min(window, _FAR), min(sinks, _FAR), 1, _kv8(k_cache), scale), q)
+    if rc:
+        _check(rc, f"klm_window_attn_prefill(T={T},S={S},window={window},sinks={sinks})")
     return out
 
 
 # ------------------------------------------------------------------ pages of a cache
+_PAGES_ARGS = struct.Struct("6P6i")             # klm_pages_args
+
+
 def _page_shape(k: torch.Tensor, v: torch.Tensor) -> Tuple[int, int, int]:
     """(layers, blocks, n_kv) of a cache [layers, blocks, n_kv, 16, 128] / [.., 128, 16], or of one layer of it."""
     if k.dim() == 4 and v.dim() == 4:
@@ -761,36 +768,47 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs: Sequence[Tup
             raise KlmOpsError("copy_pages: the two caches share memory")
     if _overlap(k_cache, v_cache):
         raise KlmOpsError("copy_pages: K and V share memory")
-    _same_device("copy_pages", k_cache, v_cache, k_src, v_src)
-    elem = k_cache.element_size()
+    if not k_cache.device == v_cache.device == k_src.device == v_src.device:
+        raise KlmOpsError("copy_pages: tensors on different devices")
     if k_cache.is_cuda:
         _kv8(k_cache)
-    p = np.asarray(pairs, dtype=np.int64).reshape(-1, 2)
+    p = _page_pairs(pairs, src_nb, nb, same)
     if not len(p):
         return
-    src, dst = p[:, 0], p[:, 1]
-    if src.min() < -1 or src.max() >= src_nb or dst.min() < 0 or dst.max() >= nb:
-        raise KlmOpsError(f"copy_pages: a pair outside the caches ({src_nb} and {nb} blocks; -1 clears)")
-    if len(np.unique(dst)) != len(dst):
-        raise KlmOpsError("copy_pages: a page is written twice")
-    if same:
-        p = p[src != dst]
-        if len(np.intersect1d(p[:, 0], dst)):
-            raise KlmOpsError("copy_pages: a page is written by one pair and read by another")
-        if not len(p):
-            return
     if not k_cache.is_cuda:
         ref.copy_pages(k_cache, v_cache, p, k_src, v_src)
         return
-    p = np.ascontiguousarray(p, dtype=np.int32)
-    with _launch_on(k_cache):
-        rc = _lib().klm_copy_pages(k_src.data_ptr(), v_src.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p.ctypes.data, len(p),
-                                   L, src_nb, nb, n_kv, elem, _stream(k_cache))
-    _check(rc, f"klm_copy_pages(pairs={len(p)},layers={L})")
+    rc = _call(_lib().klm_copy_pages, _PAGES_ARGS.pack(k_src.data_ptr(), v_src.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p.ctypes.data,
+                                                       _stream(k_cache), len(p), L, src_nb, nb, n_kv, k_cache.element_size()), k_cache)
+    if rc:
+        _check(rc, f"klm_copy_pages(pairs={len(p)},layers={L})")
+
+
+def _page_pairs(pairs, src_nb: int, nb: int, same: bool) -> np.ndarray:
+    """The pairs as int32 [n, 2], checked (see copy_pages), without those of a page and itself."""
+    p = np.asarray(pairs)
+    if p.size == 0:
+        return p.reshape(0, 2)
+    if p.ndim != 2 or p.shape[1] != 2 or p.dtype.kind not in "iu":
+        raise KlmOpsError(f"copy_pages: pairs of two page numbers are wanted, got {p.dtype} {p.shape}")
+    src, dst = p[:, 0], p[:, 1]
+    if src.min() < -1 or src.max() >= src_nb or dst.min() < 0 or dst.max() >= nb:
+        raise KlmOpsError(f"copy_pages: a pair outside the caches ({src_nb} and {nb} blocks; -1 clears)")
+    written = np.zeros(nb + 1, dtype=bool)                    # the place behind the last page stands for "nothing is read"
+    written[dst] = True
+    if np.count_nonzero(written) != len(p):
+        raise KlmOpsError("copy_pages: a page is written twice")
+    if same:
+        keep = src != dst
+        if not keep.all():
+            p = p[keep]
+            src = p[:, 0]
+        if written[src].any():                                # src -1 is that last place
+            raise KlmOpsError("copy_pages: a page is written by one pair and read by another")
+    return np.ascontiguousarray(p, dtype=np.int32)
 
 
 # ------------------------------------------------------------------ rules on logits
-@dataclass
 class LogitRules:
     """What `choose_tokens` does to rows of logits. R sets of rules:
 
@@ -801,58 +819,82 @@ class LogitRules:
     mask_rows int32 [R]       each set's mask (-1: none); without it set r uses mask r
     rows int32 [B]            the set that each row of logits follows (-1: none); without it row b follows set b
 
-    Ids outside the vocabulary are ignored. The tensors are read when the call runs: they may be changed between calls and
-    between replays of a captured one."""
-    history: torch.Tensor
-    prompt_lens: torch.Tensor
-    lens: torch.Tensor
-    repetition: torch.Tensor
-    frequency: torch.Tensor
-    presence: torch.Tensor
-    bias_ids: Optional[torch.Tensor] = None
-    bias_values: Optional[torch.Tensor] = None
-    mask: Optional[torch.Tensor] = None
-    mask_rows: Optional[torch.Tensor] = None
-    rows: Optional[torch.Tensor] = None
+    Ids outside the vocabulary are ignored. The tensors are read when the call runs: what they hold may be changed between calls
+    and between replays of a captured one; which tensors they are may not (make another LogitRules)."""
+
+    def __init__(self, history: torch.Tensor, prompt_lens: torch.Tensor, lens: torch.Tensor, repetition: torch.Tensor,
+                 frequency: torch.Tensor, presence: torch.Tensor, bias_ids: Optional[torch.Tensor] = None,
+                 bias_values: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                 mask_rows: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None):
+        self.__dict__.update(history=history, prompt_lens=prompt_lens, lens=lens, repetition=repetition, frequency=frequency,
+                             presence=presence, bias_ids=bias_ids, bias_values=bias_values, mask=mask, mask_rows=mask_rows, rows=rows)
+        i32, f32, R, device = torch.int32, torch.float32, lens.shape[0] if lens.dim() == 1 else -1, lens.device
+
+        def wants(name: str, t: torch.Tensor, dtype, *shape) -> None:
+            """`shape`: a number, or None for any."""
+            got = t.shape
+            if t.dtype != dtype or len(got) != len(shape) or got[0] != (shape[0] if shape[0] is not None else got[0]) or \
+                    (len(shape) > 1 and got[1] != (shape[1] if shape[1] is not None else got[1])) or not t.is_contiguous() or t.device != device:
+                raise KlmOpsError(f"LogitRules: {name} must be contiguous {dtype} {list(shape)} on {device}, is {t.dtype} {list(got)} on {t.device}")
+
+        # the usual case in one expression; where it does not hold, the first that is wrong is named
+        one = (R,)
+        if not (lens.dtype is i32 and prompt_lens.dtype is i32 and history.dtype is i32 and lens.shape == one == prompt_lens.shape and
+                repetition.dtype is f32 and frequency.dtype is f32 and presence.dtype is f32 and len(history.shape) == 2 and history.shape[0] == R and
+                repetition.shape == one == frequency.shape and presence.shape == one and history.is_contiguous() and
+                lens.is_contiguous() and prompt_lens.is_contiguous() and repetition.is_contiguous() and frequency.is_contiguous() and
+                presence.is_contiguous() and device == history.device == prompt_lens.device == repetition.device == frequency.device == presence.device):
+            wants("lens", lens, i32, R)
+            wants("prompt_lens", prompt_lens, i32, R)
+            wants("history", history, i32, R, None)
+            wants("repetition", repetition, f32, R)
+            wants("frequency", frequency, f32, R)
+            wants("presence", presence, f32, R)
+        if (bias_ids is None) != (bias_values is None):
+            raise KlmOpsError("LogitRules: bias_ids and bias_values go together")
+        if bias_ids is not None:
+            wants("bias_ids", bias_ids, i32, R, None)
+            wants("bias_values", bias_values, f32, R, bias_ids.shape[1])
+        if mask is not None:
+            wants("mask", mask, i32, None, None)
+            if mask_rows is not None:
+                wants("mask_rows", mask_rows, i32, R)
+            elif mask.shape[0] < R:
+                raise KlmOpsError(f"LogitRules: {mask.shape[0]} masks for {R} sets of rules and no mask_rows")
+        elif mask_rows is not None:
+            raise KlmOpsError("LogitRules: mask_rows without a mask")
+        if rows is not None:
+            wants("rows", rows, i32, None)
+
+    def __setattr__(self, name, value):
+        if value is not self.__dict__.get(name):             # `rules.lens += 1` sets the same tensor again
+            raise AttributeError("LogitRules keeps the tensors it was made with: make another one")
 
     def check(self, B: int, vocab_end: int, device) -> None:
-        R = self.lens.shape[0]
-        i32, f32 = torch.int32, torch.float32
-
-        def bad(name: str, t: torch.Tensor, shape, dtype) -> bool:
-            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-                raise KlmOpsError(f"LogitRules: {name} must be contiguous {dtype} {list(shape)} on {device}, is {t.dtype} "
-                                  f"{list(t.shape)} on {t.device}")
-            return False
-
-        if self.history.dim() != 2:
-            raise KlmOpsError("LogitRules: history must be [R, n]")
-        bad("history", self.history, (R, self.history.shape[1]), i32)
-        bad("prompt_lens", self.prompt_lens, (R,), i32)
-        bad("lens", self.lens, (R,), i32)
-        for name in ("repetition", "frequency", "presence"):
-            bad(name, getattr(self, name), (R,), f32)
-        if (self.bias_ids is None) != (self.bias_values is None):
-            raise KlmOpsError("LogitRules: bias_ids and bias_values go together")
-        if self.bias_ids is not None:
-            if self.bias_ids.dim() != 2:
-                raise KlmOpsError("LogitRules: bias_ids must be [R, k]")
-            bad("bias_ids", self.bias_ids, (R, self.bias_ids.shape[1]), i32)
-            bad("bias_values", self.bias_values, tuple(self.bias_ids.shape), f32)
-        if self.mask is not None:
-            if self.mask.dim() != 2 or self.mask.shape[1] * 32 < vocab_end:
-                raise KlmOpsError(f"LogitRules: mask {tuple(self.mask.shape)} has no bit for each of {vocab_end} tokens")
-            bad("mask", self.mask, tuple(self.mask.shape), i32)
-            if self.mask_rows is not None:
-                bad("mask_rows", self.mask_rows, (R,), i32)
-            elif self.mask.shape[0] < R:
-                raise KlmOpsError(f"LogitRules: {self.mask.shape[0]} masks for {R} sets of rules and no mask_rows")
-        elif self.mask_rows is not None:
-            raise KlmOpsError("LogitRules: mask_rows without a mask")
+        """Do these rules fit B rows of logits up to token `vocab_end`?"""
+        if self.lens.device != device:
+            raise KlmOpsError(f"LogitRules on {self.lens.device}, logits on {device}")
+        if self.mask is not None and self.mask.shape[1] * 32 < vocab_end:
+            raise KlmOpsError(f"LogitRules: mask {tuple(self.mask.shape)} has no bit for each of {vocab_end} tokens")
         if self.rows is not None:
-            bad("rows", self.rows, (B,), i32)
-        elif R < B:
-            raise KlmOpsError(f"LogitRules: {R} sets of rules for {B} rows of logits and no `rows`")
+            if self.rows.shape[0] != B:
+                raise KlmOpsError(f"LogitRules: `rows` for {self.rows.shape[0]} rows of logits, not {B}")
+        elif self.lens.shape[0] < B:
+            raise KlmOpsError(f"LogitRules: {self.lens.shape[0]} sets of rules for {B} rows of logits and no `rows`")
+
+    def _packed(self) -> Tuple[tuple, tuple]:
+        """(addresses, sizes) as klm_logits_args has them."""
+        def at(t: Optional[torch.Tensor]) -> int:
+            return 0 if t is None else t.data_ptr()
+
+        n_masks, words = (0, 0) if self.mask is None else self.mask.shape
+        return ((at(self.rows), self.history.data_ptr(), self.prompt_lens.data_ptr(), self.lens.data_ptr(), self.repetition.data_ptr(),
+                 self.frequency.data_ptr(), self.presence.data_ptr(), at(self.bias_ids), at(self.bias_values), at(self.mask), at(self.mask_rows)),
+                (self.lens.shape[0], self.history.shape[1], 0 if self.bias_ids is None else self.bias_ids.shape[1], n_masks, words))
+
+
+_LOGITS_ARGS = struct.Struct("17Pq10i")          # klm_logits_args
+_NO_RULES = (0,) * 11, (0,) * 5
 
 
 def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, first_token: int = 0,
@@ -886,26 +928,17 @@ def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, firs
         if out is not None:
             out.copy_(y)
         return ids, best
-    ids = torch.empty(B, dtype=torch.int64, device=logits.device)
-    best = torch.empty(B, dtype=torch.float32, device=logits.device)
+    ids = logits.new_empty((B,), dtype=torch.int64)
+    best = logits.new_empty((B,), dtype=torch.float32)
     if B == 0:
         return ids, best
     lib = _lib()
-    part = torch.empty((B, lib.klm_logits_parts(B, V)), dtype=torch.int64, device=logits.device)
-    r = rules
-
-    def ptr(t: Optional[torch.Tensor]):
-        return None if t is None else t.data_ptr()
-
-    if r is None:
-        args = (None, 0, None, 0, None, None, None, None, None, None, None, 0, None, 0, 0, None)
-    else:
-        args = (ptr(r.rows), r.lens.shape[0], r.history.data_ptr(), r.history.shape[1], r.prompt_lens.data_ptr(), r.lens.data_ptr(),
-                r.repetition.data_ptr(), r.frequency.data_ptr(), r.presence.data_ptr(), ptr(r.bias_ids), ptr(r.bias_values),
-                0 if r.bias_ids is None else r.bias_ids.shape[1], ptr(r.mask), 0 if r.mask is None else r.mask.shape[0],
-                0 if r.mask is None else r.mask.shape[1], ptr(r.mask_rows))
-    with _launch_on(logits):
-        rc = lib.klm_choose_tokens(logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0) if B > 1 else V, B, V, first_token, *args,
-                                   ptr(out), part.data_ptr(), ids.data_ptr(), best.data_ptr(), _stream(logits))
-    _check(rc, f"klm_choose_tokens(B={B},V={V})")
+    part = logits.new_empty((B * lib.klm_logits_parts(B, V),), dtype=torch.int64)
+    at, sizes = _NO_RULES if rules is None else rules._packed()
+    rc = _call(lib.klm_choose_tokens,
+               _LOGITS_ARGS.pack(logits.data_ptr(), *at, 0 if out is None else out.data_ptr(), part.data_ptr(), ids.data_ptr(), best.data_ptr(),
+                                 _stream(logits), logits.stride(0) if B > 1 else V, logits.dtype == torch.float32, B, V, first_token, *sizes, 0),
+               logits)
+    if rc:
+        _check(rc, f"klm_choose_tokens(B={B},V={V})")
     return ids, best
