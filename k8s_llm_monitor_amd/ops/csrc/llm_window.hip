@@ -13,8 +13,6 @@
 
 using namespace klm_llm;
 
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-
 namespace {
 
 struct WinArgs {
@@ -281,62 +279,74 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, size_t n_he
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Prompts and chunks of prompts. Query rows are (token, head of the kv head's group) pairs in a row; a block takes 128 * QT
-// of them (4 waves of QT 32-row tiles) and walks the 32-key steps they may see, staged through LDS as bf16.
-//   S^T = K Q^T with v_mfma_f32_32x32x16_bf16: first operand lane l = row l%32, k = (l/32)*8 ..+8; result lane l = column
-//   (query row) l%32, register i = row 8*(i/4) + 4*(l/32) + i%4. Row r of the K operand holds token
-//   16*(r/16) + 8*bit2(r) + 4*bit3(r) + r%4, so that lane l ends up with the scores of tokens 8*(l/32) .. +8 of page 0
-//   (registers 0..7) and of page 1 (8..15): the second operand that O^T = V^T P wants from it, no value changes lanes.
-// LDS step: K [32 tokens][16 chunks of 16 bytes], chunk c of token t at c ^ key(t); V [page][dims/32][half][dims%32] chunks of
-// 8 tokens, so that a fragment is 1 KiB in lane order.
+// Prompts and chunks of prompts. Query rows are (token, head of the kv head's group) pairs in a row; a wave takes QT tiles of
+// 16 of them, a block of 4 waves walks the 32-key steps they may see, staged through LDS as bf16. The operand mapping is
+// decode's (and llm_attention.hip's): lane (fr, fq) has query row fr and, after S^T = K Q^T, the scores of keys fq*8 .. + 7;
+// these are the second operand that O^T = V^T P wants from it, no value changes lanes.
+// LDS step: K [32 tokens][16 chunks of 16 bytes], chunk c of token t at c ^ key(t): the 16 rows of a fragment read 16 chunk
+// columns. V [dims/16][fq][dims%16] chunks of 8 tokens: a fragment is 1 KiB in lane order. A ring of 4 steps; a bf16 cache is
+// brought in by LDS-DMA three steps ahead (4 KiB a wave, no registers), an e4m3 cache through registers, where it becomes
+// bf16 once per block.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int STEP_BYTES = 16384;
+#ifndef QTILES
+#define QTILES 3
+#endif
+constexpr int STEP_BYTES = 16384, RING = 4;
 
-__device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) & 1) << 2) | (((tok >> 2) & 1) << 3); }
+__device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) & 3) << 2); }
 
-template <bool KV8>
-struct Stage {
-  uint4 r[KV8 ? 2 : 4];
+#define KLM_AS1 __attribute__((address_space(1)))
+#define KLM_AS3 __attribute__((address_space(3)))
+#define KLM_AS4 __attribute__((address_space(4)))
+__device__ __forceinline__ void glds16(const void* g, void* lds) {
+  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)g, (KLM_AS3 void*)lds, 16, 0, 0);
+}
+
+struct Pages2 {
+  int p0, p1;            // a step's two pages, -1: none
 };
+// through the scalar cache: the index is the same in all lanes, and the vector memory counter stays with the DMA
+__device__ __forceinline__ Pages2 pages_of(const int* table, int step, int width, int pages) {
+  const KLM_AS4 int* t = (const KLM_AS4 int*)table;
+  const int i0 = step * 2, i1 = step * 2 + 1;
+  const int a = t[i0 < width ? i0 : width - 1], b = t[i1 < width ? i1 : width - 1];
+  return Pages2{(i0 < width && a >= 0 && a < pages) ? a : -1, (i1 < width && b >= 0 && b < pages) ? b : -1};
+}
 
-template <bool KV8>
-__device__ __forceinline__ void stage_load(const WinArgs& a, const int* table, int h, int step, int tid, Stage<KV8>& s) {
-  const int p0 = page_at(table, step * 2, a.width, a.pages), p1 = page_at(table, step * 2 + 1, a.width, a.pages);
-  const size_t b0 = ((size_t)(p0 < 0 ? 0 : p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(p1 < 0 ? 0 : p1) * a.n_kv + h) * BLK_ELEMS;
-  if (KV8) {
-    const size_t o = ((tid >> 7) ? b1 : b0) + (tid & 127) * 16;
-    s.r[0] = *reinterpret_cast<const uint4*>((const uint8_t*)a.kc + o);
-    s.r[1] = *reinterpret_cast<const uint4*>((const uint8_t*)a.vc + o);
-  } else {
-    const int e = tid * 8;
-    s.r[0] = *reinterpret_cast<const uint4*>((const uint16_t*)a.kc + b0 + e);
-    s.r[1] = *reinterpret_cast<const uint4*>((const uint16_t*)a.kc + b1 + e);
-    s.r[2] = *reinterpret_cast<const uint4*>((const uint16_t*)a.vc + b0 + e);
-    s.r[3] = *reinterpret_cast<const uint4*>((const uint16_t*)a.vc + b1 + e);
+__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, char* st, int w, int lane) {
+  const size_t b0 = ((size_t)(pg.p0 < 0 ? 0 : pg.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(pg.p1 < 0 ? 0 : pg.p1) * a.n_kv + h) * BLK_ELEMS;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int p = 2 * w + j;                         // piece: K tokens 4p .. 4p + 3; V dims 16p .. + 15
+    const int tok = p * 4 + (lane >> 4);
+    glds16((const uint16_t*)a.kc + (p >= 4 ? b1 : b0) + (tok & 15) * HD + (((lane & 15) ^ k_key(tok)) << 3), st + p * 1024);
+    glds16((const uint16_t*)a.vc + (lane >= 32 ? b1 : b0) + (p * 16 + (lane & 15)) * BLK + ((lane >> 4) & 1) * 8, st + 8192 + p * 1024);
   }
 }
 
-template <bool KV8>
-__device__ __forceinline__ void stage_store(char* st, int tid, const Stage<KV8>& s) {
-  if (KV8) {
-    const int tok = tid >> 3, c = (tid & 7) * 2, key = k_key(tok & 15);
-    char* kp = st + tok * 256;
-    *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(s.r[0].x, s.r[0].y);
-    *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(s.r[0].z, s.r[0].w);
-    const int page = tid >> 7, dim = tid & 127;
-    char* vp = st + 8192 + page * 4096 + (dim >> 5) * 1024 + (dim & 31) * 16;
-    *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(s.r[1].x, s.r[1].y);
-    *reinterpret_cast<bf16x8*>(vp + 512) = fp8x8_to_bf16(s.r[1].z, s.r[1].w);
-  } else {
-    const int tok = tid >> 4, c = tid & 15;
-    const int ko = tok * 256 + ((c ^ k_key(tok)) << 4);
-    *reinterpret_cast<uint4*>(st + ko) = s.r[0];
-    *reinterpret_cast<uint4*>(st + 4096 + ko) = s.r[1];
-    const int dim = tid >> 1, half = tid & 1;
-    char* vp = st + 8192 + (dim >> 5) * 1024 + half * 512 + (dim & 31) * 16;
-    *reinterpret_cast<uint4*>(vp) = s.r[2];
-    *reinterpret_cast<uint4*>(vp + 4096) = s.r[3];
-  }
+struct Stage8 {
+  uint4 k, v;
+};
+__device__ __forceinline__ void stage8_load(const WinArgs& a, Pages2 pg, int h, int tid, Stage8& s) {
+  const int id = (tid >> 7) ? pg.p1 : pg.p0;
+  const size_t o = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * BLK_ELEMS + (tid & 127) * 16;
+  s.k = *reinterpret_cast<const uint4*>((const uint8_t*)a.kc + o);
+  s.v = *reinterpret_cast<const uint4*>((const uint8_t*)a.vc + o);
+}
+__device__ __forceinline__ void stage8_store(char* st, int tid, const Stage8& s) {
+  const int tok = tid >> 3, c = (tid & 7) * 2, key = k_key(tok);
+  char* kp = st + tok * 256;
+  *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(s.k.x, s.k.y);
+  *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(s.k.z, s.k.w);
+  const int page = tid >> 7, dim = tid & 127;
+  char* vp = st + 8192 + (dim >> 4) * 1024 + page * 512 + (dim & 15) * 16;
+  *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(s.v.x, s.v.y);
+  *reinterpret_cast<bf16x8*>(vp + 256) = fp8x8_to_bf16(s.v.z, s.v.w);
+}
+
+// a row of seq_info that counts: queries inside q, and a context that holds them (rows * G fits 31 bits, see the launcher)
+__device__ __forceinline__ bool is_sequence(const WinArgs& a, int q_start, int q_len, int ctx) {
+  return q_len > 0 && ctx >= q_len && q_start >= 0 && q_len <= a.rows && q_start <= a.rows - q_len;
 }
 
 // tile t of the launch -> its sequence and its number among the sequence's tiles; false: the launch has more tiles than needed
@@ -346,8 +356,8 @@ __device__ __forceinline__ bool find_tile(const WinArgs& a, int rows, int t, int
     const int i = s0 + lane;
     int n = 0;
     if (i < a.n_seqs) {
-      const int ql = a.lens[i * 3 + 1], cl = a.lens[i * 3 + 2];
-      if (ql > 0 && cl >= ql) n = (int)(((int64_t)ql * a.G + rows - 1) / rows);
+      const int qs = a.lens[i * 3], ql = a.lens[i * 3 + 1], cl = a.lens[i * 3 + 2];
+      if (is_sequence(a, qs, ql, cl)) n = (int)(((unsigned)(ql * a.G) + rows - 1) / rows);
     }
     int inc = n;
 #pragma unroll
@@ -369,192 +379,316 @@ __device__ __forceinline__ bool find_tile(const WinArgs& a, int rows, int t, int
   return false;
 }
 
+// A wave's state: QT tiles of 16 query rows, lane (fr, fq) has row fr of each.
+template <int QT>
+struct Rows {
+  bf16x8 q[QT][4];
+  f32x4 o[QT][8];
+  float m[QT], shift[QT], l[QT];       // the maximum that weights are relative to (scaled, log2), minus it (0 while unset), their sum
+  int pos[QT];
+};
+
+// Marks a NaN with 4096, +inf with 1, -inf with 64, all else with 0, as two bf16 numbers.
+__device__ __forceinline__ uint32_t odd_marks(uint32_t x) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t e = (x >> (16 * i)) & 0xffffu;
+    const uint32_t mark = (e & 0x7f80u) != 0x7f80u ? 0u : (e & 0x7fu) ? 0x4580u : (e >> 15) ? 0x4280u : 0x3f80u;
+    r |= mark << (16 * i);
+  }
+  return r;
+}
+
+// One 32-key step for the wave's rows. inside (wave-uniform): every row in use sees every key of the step.
+template <int QT>
+__device__ __forceinline__ void prefill_step(const WinArgs& a, const char* st, int step, Pages2 pg, bool inside, int lane, Rows<QT>& r, bool& odd) {
+  const int fr = lane & 15, fq = lane >> 4;
+  const char* kp = st + ((fr >> 2) * 8 + (fr & 3)) * 256;              // k_key of both tokens below is fr
+  f32x4 s[QT][2];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
+    const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s[t][0], 0, 0, 0);
+      s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s[t][1], 0, 0, 0);
+    }
+  }
+  const int key = step * 32 + fq * 8;                                  // the lane's scores: keys key .. + 7, of one page
+  const bool page = ((fq >> 1) ? pg.p1 : pg.p0) >= 0;
+  bf16x8 p[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = s[t][0][j];
+      x[j + 4] = s[t][1][j];
+    }
+    if (!inside) {
+      const int up = page ? r.pos[t] - key : -1, down = r.pos[t] - key - a.window, sink = a.sinks - key;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j <= up && (j > down || j < sink) ? x[j] : -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    // The weights are relative to a maximum that is moved only when a score passes it by 8 (a weight of 256): their ratio to
+    // the sum is what counts, and bf16 keeps it at any size. Most steps then need nothing from another lane.
+    if (__ballot(mx * a.scale_log2 > r.m[t] + 8.f) != 0) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(r.m[t], mx * a.scale_log2);
+      const float shift = m_new == -INFINITY ? 0.f : -m_new;
+      const float alpha = fast_exp2(r.m[t] + shift);
+      r.m[t] = m_new;
+      r.shift[t] = shift;
+      r.l[t] *= alpha;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) r.o[t][n] *= alpha;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float pj = fast_exp2(fmaf(x[j], a.scale_log2, r.shift[t]));
+      p[t][j] = (__bf16)pj;
+      sum += pj;
+    }
+    r.l[t] += sum;
+  }
+  const char* vp = st + 8192 + lane * 16;
+  // A row that does not see a key has weight 0 for it, and 0 times a NaN or an infinity in V would be NaN: a step at the edge
+  // that holds such values sends the wave's rows to careful_tile.
+  if (!inside) {
+    uint32_t any = 0;
+#pragma unroll 2                                                       // not more: registers
+    for (int n = 0; n < 8; ++n) {
+      const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 1024);
+      any |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
+    }
+    odd = odd || __ballot(any != 0) != 0;
+  }
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 1024);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
+  }
+}
+
+// The finished rows of one 16-row tile: lane (fr, fq) holds dims n * 16 + fq * 4 .. + 3 of row fr; dst < 0: no row.
+__device__ __forceinline__ void write_rows(const WinArgs& a, int64_t dst, int split, int fq, const f32x4 (&o)[8], float m, float l) {
+  if (dst < 0) return;
+  if (a.splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      bf16x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (__bf16)(o[n][j] * inv);
+      *reinterpret_cast<bf16x4*>(a.out + dst * HD + n * 16 + fq * 4) = v;
+    }
+  } else {
+    const size_t at = (size_t)dst * a.splits + split;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4*>(a.part_o + at * HD + n * 16 + fq * 4) = o[n];
+    if (fq == 0) {
+      a.part_ml[at * 2] = m;
+      a.part_ml[at * 2 + 1] = l;
+    }
+  }
+}
+
+// One 16-row tile again, from the cache and by itself, where V holds NaN or infinities that some rows see and others do not:
+// they leave the matrix product, and the rows that see them get them back. Rare and slow: a wave's steps one after another.
+template <bool KV8>
+__device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table, int h, const Span& sp, int i0, int i1, int split, int lane,
+                                             const uint16_t* qrow, int pos, int64_t dst) {
+  const int fr = lane & 15, fq = lane >> 4;
+  bf16x8 q[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    uint4 u = uint4{0, 0, 0, 0};
+    if (dst >= 0) u = *reinterpret_cast<const uint4*>(qrow + (KV8 ? (s >> 1) * 64 + fq * 16 + (s & 1) * 8 : s * 32 + fq * 8));
+    q[s] = __builtin_bit_cast(bf16x8, u);
+  }
+  f32x4 o[8];
+#pragma unroll
+  for (int n = 0; n < 8; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int i = i0; i < i1; ++i) {
+    const int step = sp.step(i), key = step * 32 + fq * 8;
+    DFrags f;
+    load_step<KV8>(a, table, h, step, fr, fq, f);
+    f32x4 s0 = f32x4{0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[0][s], q[s], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[1][s], q[s], s1, 0, 0, 0);
+    }
+    const int up = ((fq >> 1) ? f.p1 : f.p0) >= 0 ? pos - key : -1, down = pos - key - a.window, sink = a.sinks - key;
+    float x[8], mx = -INFINITY;
+    uint32_t ones[4] = {0u, 0u, 0u, 0u};                               // 1 for a key that the row sees, as bf16 pairs
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool see = j <= up && (j > down || j < sink);
+      x[j] = see ? (j < 4 ? s0[j & 3] : s1[j & 3]) : -INFINITY;
+      ones[j >> 1] |= see ? 0x3f80u << (16 * (j & 1)) : 0u;
+      mx = fmaxf(mx, x[j]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float m_new = fmaxf(m, mx * a.scale_log2), shift = m_new == -INFINITY ? 0.f : -m_new;
+    const float alpha = fast_exp2(m + shift);
+    m = m_new;
+    l *= alpha;
+    bf16x8 p;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float pj = fast_exp2(fmaf(x[j], a.scale_log2, shift));
+      p[j] = (__bf16)pj;
+      l += pj;
+    }
+    const bf16x8 one = __builtin_bit_cast(bf16x8, uint4{ones[0], ones[1], ones[2], ones[3]});
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      uint4 u = __builtin_bit_cast(uint4, f.v[n]);
+      const uint4 marks = uint4{odd_marks(u.x), odd_marks(u.y), odd_marks(u.z), odd_marks(u.w)};
+      // how many of them each row sees in each dim: exact in fp32
+      const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, marks), one, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      u = uint4{without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w)};
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u), p, o[n] * alpha, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int all = (int)c[j], neg = (all >> 6) & 63, inf = all & 63;
+        o[n][j] += all >= 4096 || (neg && inf) ? NAN : neg ? -INFINITY : inf ? INFINITY : 0.f;
+      }
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  write_rows(a, dst, split, fq, o, m, l);
+}
+
 template <int QT, bool KV8>
-__global__ __launch_bounds__(256) void window_prefill_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int h = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, hi = lane >> 5;
-  constexpr int ROWS = 128 * QT;
+  const int fr = lane & 15, fq = lane >> 4;
+  constexpr int ROWS = 64 * QT;
   int seq, tile;
   if (!find_tile(a, ROWS, blockIdx.y, lane, seq, tile)) return;
   const int q_start = a.lens[seq * 3], q_len = a.lens[seq * 3 + 1], ctx = a.lens[seq * 3 + 2];
   const int* table = a.tables + (size_t)seq * a.width;
   const int first = ctx - q_len;                                       // position of the sequence's first query
-  const int64_t r0 = (int64_t)tile * ROWS;
-  const int tok_a = (int)(r0 / a.G);
-  const int64_t tb = (r0 + ROWS - 1) / a.G;
-  const int tok_b = tb < q_len ? (int)tb : q_len - 1;
+  const unsigned G = a.G, r0 = (unsigned)tile * ROWS;
+  const int tok_a = r0 / G, tb = (r0 + ROWS - 1) / G, tok_b = tb < q_len ? tb : q_len - 1;
   const Span sp = make_span(first + tok_a, first + tok_b, a.window, a.sinks, a.width);
   const int sps = (sp.n + a.splits - 1) / a.splits;
   const int i0 = split * sps, i1 = (i0 + sps) < sp.n ? (i0 + sps) : sp.n;
 
-  bf16x8 qf[QT][8];
-  f32x16 o[QT][4];
-  float m[QT], l[QT];
-  int pos[QT];
-  int64_t dst[QT];
-  int pmin[QT], pmax[QT];
+  Rows<QT> r;
+  // row fr of tile t: its token (>= q_len: none) and head of the group
+  const auto row_of = [&](int t, int& token, int& g) {
+    const unsigned R = r0 + (w * QT + t) * 16 + fr;
+    token = R / G;
+    g = R - (unsigned)token * G;
+  };
+  const unsigned ra = r0 + w * QT * 16;                                // the wave's first and last position; of no rows: nothing is inside
+  const int ta = ra / G, tz = (ra + QT * 16 - 1) / G;
+  const int pmin = ta < q_len ? first + ta : -1, pmax = first + (tz < q_len ? tz : q_len - 1);
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const int64_t R = r0 + (w * QT + t) * 32;
-    const int64_t tq = (R + col) / a.G;
-    const int g = (int)((R + col) % a.G);
-    const int64_t qrow = q_start + tq;
-    const bool valid = tq < q_len && qrow >= 0 && qrow < a.rows;
-    pos[t] = valid ? first + (int)tq : -1;
-    dst[t] = valid ? (qrow * a.n_q + (int64_t)h * a.G + g) : -1;
-    const uint16_t* qp = a.q + (valid ? qrow * a.q_stride + ((int64_t)h * a.G + g) * HD : 0);
+    int token, g;
+    row_of(t, token, g);
+    const bool valid = token < q_len;
+    r.pos[t] = valid ? first + token : -1;                             // a row that is none sees nothing
+    const uint16_t* qp = a.q + (valid ? (size_t)(q_start + token) * a.q_stride + ((size_t)h * G + g) * HD : 0);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      if (valid) qf[t][s] = *reinterpret_cast<const bf16x8*>(qp + s * 16 + hi * 8);
+    for (int s = 0; s < 4; ++s) {
+      if (valid) r.q[t][s] = *reinterpret_cast<const bf16x8*>(qp + s * 32 + fq * 8);
       else
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qf[t][s][j] = (__bf16)0.f;
+        for (int j = 0; j < 8; ++j) r.q[t][s][j] = (__bf16)0.f;
     }
-    const int64_t ta = R / a.G, tz = (R + 31) / a.G;                   // wave-uniform: the tile's first and last position
-    pmin[t] = ta < q_len ? first + (int)ta : 0x7fffffff;               // past the queries: sees nothing, skips every step
-    pmax[t] = ta < q_len ? first + (int)(tz < q_len ? tz : q_len - 1) : -1;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[t][n][i] = 0.f;
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+    for (int n = 0; n < 8; ++n) r.o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    r.m[t] = -INFINITY;
+    r.shift[t] = 0.f;
+    r.l[t] = 0.f;
   }
 
-  Stage<KV8> sg;
-  if (i0 < i1) stage_load<KV8>(a, table, h, sp.step(i0), tid, sg);
-  for (int i = i0; i < i1; ++i) {
-    char* st = lds + ((i - i0) & 1) * STEP_BYTES;
-    stage_store<KV8>(st, tid, sg);
-    if (i + 1 < i1) stage_load<KV8>(a, table, h, sp.step(i + 1), tid, sg);
-    __syncthreads();
-    const int step = sp.step(i), k0 = step * 32;
-    const int pg0 = page_at(table, step * 2, a.width, a.pages), pg1 = page_at(table, step * 2 + 1, a.width, a.pages);
+  bool odd = false;
+  if (i0 < i1) {
+    // pages of the step that is computed, and of the steps that are on their way
+    Pages2 pg[RING];
+    Stage8 sg;
+    const int last = i1 - 1;
+    if (KV8) {
+      pg[0] = pages_of(table, sp.step(i0), a.width, a.pages);
+      stage8_load(a, pg[0], h, tid, sg);
+      stage8_store(lds, tid, sg);
+      pg[1] = pages_of(table, sp.step(i0 + 1 < i1 ? i0 + 1 : last), a.width, a.pages);
+      stage8_load(a, pg[1], h, tid, sg);
+      pg[2] = pages_of(table, sp.step(i0 + 2 < i1 ? i0 + 2 : last), a.width, a.pages);
+    } else {
 #pragma unroll
+      for (int j = 0; j < RING - 1; ++j) {
+        pg[j] = pages_of(table, sp.step(i0 + j < i1 ? i0 + j : last), a.width, a.pages);
+        dma_step(a, pg[j], h, lds + j * STEP_BYTES, w, lane);
+      }
+    }
+    pg[3] = pages_of(table, sp.step(i0 + 3 < i1 ? i0 + 3 : last), a.width, a.pages);
+    for (int i = i0; i < i1; ++i) {
+      const int at = i - i0;
+      if (KV8) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // this wave's part of step i is in LDS
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        stage8_store(lds + ((at + 1) & (RING - 1)) * STEP_BYTES, tid, sg);
+        stage8_load(a, pg[2], h, tid, sg);
+      } else {
+        // 4 DMA instructions a wave and step, in order: at most those of the two newer steps may be on their way
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        dma_step(a, pg[3], h, lds + ((at + 3) & (RING - 1)) * STEP_BYTES, w, lane);
+      }
+      const int step = sp.step(i), k0 = step * 32;
+      const Pages2 now = pg[0];
+      pg[0] = pg[1]; pg[1] = pg[2]; pg[2] = pg[3];
+      pg[3] = pages_of(table, sp.step(i + 4 < i1 ? i + 4 : last), a.width, a.pages);
+      const char* st = lds + (at & (RING - 1)) * STEP_BYTES;
+      const bool inside = k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && now.p0 >= 0 && now.p1 >= 0;
+      prefill_step<QT>(a, st, step, now, inside, lane, r, odd);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // the last, unused steps land before the LDS goes away
+  }
+
+  if (odd) {
+#pragma unroll 1
     for (int t = 0; t < QT; ++t) {
-      // does any row of the tile see a key of this step?
-      if (k0 > pmax[t] || (k0 + 31 <= pmin[t] - a.window && k0 >= a.sinks)) continue;
-      f32x16 s;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = 0.f;
-      const int tok = (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
-      const char* kp = st + tok * 256;
-      const int key = k_key(tok & 15);
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(kp + (((c * 2 + hi) ^ key) << 4)), qf[t][c], s, 0, 0, 0);
-      const bool inside = k0 + 31 <= pmin[t] && (k0 > pmax[t] - a.window || k0 + 31 < a.sinks) && pg0 >= 0 && pg1 >= 0;
-      if (!inside) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int k = k0 + (j >> 3) * 16 + hi * 8 + (j & 7);
-          const bool see = k <= pos[t] && (k > pos[t] - a.window || k < a.sinks) && ((j >> 3) ? pg1 : pg0) >= 0;
-          s[j] = see ? s[j] : -INFINITY;
-        }
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m[t], mx * a.scale_log2);
-      const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
-      const float alpha = fast_exp2(m[t] - m_use);
-      bf16x8 p[2];
-      float rs = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float pj = fast_exp2(fmaf(s[j], a.scale_log2, -m_use));
-        p[j >> 3][j & 7] = (__bf16)pj;
-        rs += pj;
-      }
-      l[t] = l[t] * alpha + rs;
-      m[t] = m_new;
-      if (__ballot(alpha != 1.f) != 0) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) o[t][n] *= alpha;
-      }
-      // Some row of the tile may not see a key whose V holds a NaN or an infinity: 0 times that would be NaN. Such values
-      // are taken out of the matrix product and added for the rows that do see them.
-      uint32_t odd = 0;
-      bf16x8 vf[4][2];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) vf[n][g] = *reinterpret_cast<const bf16x8*>(st + 8192 + g * 4096 + n * 1024 + lane * 16);
-      if (!inside) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const uint4 u = __builtin_bit_cast(uint4, vf[n][g]);
-            odd |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
-          }
-        if (__ballot(odd != 0) != 0) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              uint4 u = __builtin_bit_cast(uint4, vf[n][g]);
-              u = uint4{without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w)};
-              vf[n][g] = __builtin_bit_cast(bf16x8, u);
-            }
-          for (int kk = 0; kk < 32; ++kk) {                            // (page, half, token): register (page, token) of lane half
-            const int pg = kk >> 4, half = (kk >> 3) & 1, e = kk & 7;
-            float pk = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) pk = (pg * 8 + e) == j ? (float)p[j >> 3][j & 7] : pk;
-            pk = __shfl(pk, col + half * 32);
-            const int k = k0 + kk;
-            const bool see = k <= pos[t] && (k > pos[t] - a.window || k < a.sinks) && (pg ? pg1 : pg0) >= 0;
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-              for (int i2 = 0; i2 < 16; ++i2) {
-                const int d = 8 * (i2 >> 2) + 4 * hi + (i2 & 3);
-                const uint16_t e16 = *reinterpret_cast<const uint16_t*>(st + 8192 + pg * 4096 + n * 1024 + half * 512 + d * 16 + e * 2);
-                if (see && (e16 & 0x7f80) == 0x7f80) o[t][n][i2] += pk * bf2f(e16);
-              }
-          }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) o[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n][g], p[g], o[t][n], 0, 0, 0);
+      int token, g;
+      row_of(t, token, g);
+      const bool valid = token < q_len;
+      const size_t row = q_start + (valid ? token : 0), head = (size_t)h * G + g;
+      careful_tile<KV8>(a, table, h, sp, i0, i1, split, lane, a.q + row * a.q_stride + head * HD, valid ? first + token : -1,
+                        valid ? (int64_t)(row * a.n_q + head) : -1);
     }
+    return;
   }
-
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    l[t] += __shfl_xor(l[t], 32);
-    if (dst[t] < 0) continue;
-    if (a.splits == 1) {
-      const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bf16x4 v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = (__bf16)(o[t][n][i * 4 + j] * inv);
-          *reinterpret_cast<bf16x4*>(a.out + dst[t] * HD + n * 32 + i * 8 + hi * 4) = v;
-        }
-    } else {
-      const size_t at = (size_t)dst[t] * a.splits + split;
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f32x4*>(a.part_o + at * HD + n * 32 + i * 8 + hi * 4) =
-              f32x4{o[t][n][i * 4], o[t][n][i * 4 + 1], o[t][n][i * 4 + 2], o[t][n][i * 4 + 3]};
-      if (hi == 0) {
-        a.part_ml[at * 2] = m[t];
-        a.part_ml[at * 2 + 1] = l[t];
-      }
-    }
+    r.l[t] += __shfl_xor(r.l[t], 16);
+    r.l[t] += __shfl_xor(r.l[t], 32);
+    int token, g;
+    row_of(t, token, g);
+    write_rows(a, token < q_len ? (int64_t)((size_t)(q_start + token) * a.n_q + (size_t)h * G + g) : -1, split, fq, r.o[t], r.m[t], r.l[t]);
   }
 }
 
@@ -603,12 +737,12 @@ int klm_window_attn_prefill(const klm_window_args* c) {
   const WinArgs a = device_args(c);
   const int rc = check_args(a);
   if (rc != KLM_OK) return rc;
-  const int64_t tiles = ((int64_t)a.rows * a.G + 255) / 256 + a.n_seqs;       // every sequence may end in a partial tile
-  if (tiles > 65535) return KLM_ERR_SHAPE;
+  const int64_t tiles = ((int64_t)a.rows * a.G + 64 * QTILES - 1) / (64 * QTILES) + a.n_seqs;       // every sequence may end in a partial tile
+  if (tiles > 65535 || (int64_t)a.rows * a.G > (1 << 30)) return KLM_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(c->stream);
   const dim3 grid(a.n_kv, (unsigned)tiles, 1);
-  if (c->kv_fp8) hipLaunchKernelGGL((window_prefill_kernel<2, true>), grid, dim3(256), 2 * STEP_BYTES, s, a);
-  else hipLaunchKernelGGL((window_prefill_kernel<2, false>), grid, dim3(256), 2 * STEP_BYTES, s, a);
+  if (c->kv_fp8) hipLaunchKernelGGL((window_prefill_kernel<QTILES, true>), grid, dim3(256), RING * STEP_BYTES, s, a);
+  else hipLaunchKernelGGL((window_prefill_kernel<QTILES, false>), grid, dim3(256), RING * STEP_BYTES, s, a);
   return launch_status();
 }
 

@@ -701,8 +701,9 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     last q_len tokens of a context of ctx_len that is in the cache already; seq_info int32 [S, 3] = (q_start, q_len, ctx_len).
 
     No table of tiles: the kernel finds its work in `seq_info`, so nothing is computed on the host from the lengths and a
-    captured call may be replayed with others. The sequences' rows must not overlap. Rows of no sequence (padding, or one
-    with q_len <= 0 or ctx_len < q_len) stay as they are in a given `out` and are zero otherwise."""
+    captured call may be replayed with others. The sequences' rows must not overlap. A row of seq_info with q_len <= 0,
+    ctx_len < q_len or queries that do not lie in q is no sequence. Rows of no sequence stay as they are in a given `out` and
+    are zero otherwise."""
     what = "paged_attn_prefill_window"
     _check_window(what, q, k_cache, v_cache, block_tables, seq_info, scale, n_q, window, sinks, out)
     S, width = block_tables.shape

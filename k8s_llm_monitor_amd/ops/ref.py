@@ -174,14 +174,11 @@ def window_attn_prefill(q, k_cache, v_cache, block_tables, seq_info, scale: floa
         out = torch.zeros((q.shape[0], q.shape[-1]), dtype=q.dtype, device=q.device)
     for s in range(seq_info.shape[0]):
         q0, ql, ctx = (int(x) for x in seq_info[s])
-        if ql <= 0 or ctx < ql:
+        if ql <= 0 or ctx < ql or q0 < 0 or q0 + ql > q.shape[0]:
             continue
-        lo, hi = max(0, q0), min(q0 + ql, q.shape[0])                      # rows outside q belong to nobody
-        if hi <= lo:
-            continue
-        pos = torch.arange(ctx - ql + lo - q0, ctx - ql + hi - q0, device=q.device)
-        o = _window_rows(q[lo:hi].to(dtype).view(hi - lo, -1, HEAD_DIM), k_cache, v_cache, block_tables[s], ctx, pos, scale, window, sinks)
-        out[lo:hi] = o.reshape(hi - lo, -1).to(out.dtype)
+        pos = torch.arange(ctx - ql, ctx, device=q.device)
+        o = _window_rows(q[q0:q0 + ql].to(dtype).view(ql, -1, HEAD_DIM), k_cache, v_cache, block_tables[s], ctx, pos, scale, window, sinks)
+        out[q0:q0 + ql] = o.reshape(ql, -1).to(out.dtype)
     return out
 
 
