@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, size_t n_he
 // decode's (and llm_attention.hip's): lane (fr, fq) has query row fr and, after S^T = K Q^T, the scores of keys fq*8 .. + 7;
 // these are the second operand that O^T = V^T P wants from it, no value changes lanes.
 // LDS step: K [32 tokens][16 chunks of 16 bytes], chunk c of token t at c ^ key(t): the 16 rows of a fragment read 16 chunk
-// columns. V [dims/16][fq][dims%16] chunks of 8 tokens: a fragment is 1 KiB in lane order. A ring of 4 steps; a bf16 cache is
+// columns. V [page][dims/16][half][dims%16] chunks of 8 tokens: half a wave reads 512 bytes in lane order. A ring of 4 steps; a bf16 cache is
 // brought in by LDS-DMA three steps ahead (4 KiB a wave, no registers), an e4m3 cache through registers, where it becomes
 // bf16 once per block.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -298,30 +298,30 @@ __device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) 
 #define KLM_AS1 __attribute__((address_space(1)))
 #define KLM_AS3 __attribute__((address_space(3)))
 #define KLM_AS4 __attribute__((address_space(4)))
-__device__ __forceinline__ void glds16(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)g, (KLM_AS3 void*)lds, 16, 0, 0);
-}
-
 struct Pages2 {
   int p0, p1;            // a step's two pages, -1: none
 };
-// through the scalar cache: the index is the same in all lanes, and the vector memory counter stays with the DMA
+// Through the scalar cache: the index is the same in all lanes, and the vector memory counter stays with the DMA. A step of a
+// span has its first page inside the table.
 __device__ __forceinline__ Pages2 pages_of(const int* table, int step, int width, int pages) {
   const KLM_AS4 int* t = (const KLM_AS4 int*)table;
-  const int i0 = step * 2, i1 = step * 2 + 1;
-  const int a = t[i0 < width ? i0 : width - 1], b = t[i1 < width ? i1 : width - 1];
-  return Pages2{(i0 < width && a >= 0 && a < pages) ? a : -1, (i1 < width && b >= 0 && b < pages) ? b : -1};
+  const int i1 = step * 2 + 1 < width ? step * 2 + 1 : width - 1;
+  const int a = t[step * 2], b = t[i1];
+  return Pages2{(unsigned)a < (unsigned)pages ? a : -1, (unsigned)b < (unsigned)pages && step * 2 + 1 < width ? b : -1};
 }
 
-__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, char* st, int w, int lane) {
-  const size_t b0 = ((size_t)(pg.p0 < 0 ? 0 : pg.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(pg.p1 < 0 ? 0 : pg.p1) * a.n_kv + h) * BLK_ELEMS;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int p = 2 * w + j;                         // piece: K tokens 4p .. 4p + 3; V dims 16p .. + 15
-    const int tok = p * 4 + (lane >> 4);
-    glds16((const uint16_t*)a.kc + (p >= 4 ? b1 : b0) + (tok & 15) * HD + (((lane & 15) ^ k_key(tok)) << 3), st + p * 1024);
-    glds16((const uint16_t*)a.vc + (lane >= 32 ? b1 : b0) + (p * 16 + (lane & 15)) * BLK + ((lane >> 4) & 1) * 8, st + 8192 + p * 1024);
-  }
+// A wave brings a quarter of a step, half a page: K tokens 8w .. 8w + 7 (the chunk swizzle is the same for both fours of
+// them), V dims 64 (w % 2) .. + 63; `ko`, `vo`: the lane's offsets in bytes inside the page. The second half of each lies 1 KiB
+// behind the first, in memory as in LDS.
+__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, char* st, int w, unsigned ko, unsigned vo) {
+  const int id = w < 2 ? pg.p0 : pg.p1;
+  const size_t base = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * (BLK_ELEMS * 2);
+  const char* k = (const char*)a.kc + base;
+  const char* v = (const char*)a.vc + base;
+  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(k + ko), (KLM_AS3 void*)(st + w * 2048), 16, 0, 0);
+  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(k + ko), (KLM_AS3 void*)(st + w * 2048), 16, 1024, 0);
+  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(v + vo), (KLM_AS3 void*)(st + 8192 + w * 2048), 16, 0, 0);
+  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(v + vo), (KLM_AS3 void*)(st + 8192 + w * 2048), 16, 1024, 0);
 }
 
 struct Stage8 {
@@ -339,7 +339,7 @@ __device__ __forceinline__ void stage8_store(char* st, int tid, const Stage8& s)
   *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(s.k.x, s.k.y);
   *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(s.k.z, s.k.w);
   const int page = tid >> 7, dim = tid & 127;
-  char* vp = st + 8192 + (dim >> 4) * 1024 + page * 512 + (dim & 15) * 16;
+  char* vp = st + 8192 + page * 4096 + (dim >> 4) * 512 + (dim & 15) * 16;
   *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(s.v.x, s.v.y);
   *reinterpret_cast<bf16x8*>(vp + 256) = fp8x8_to_bf16(s.v.z, s.v.w);
 }
@@ -365,13 +365,11 @@ __device__ __forceinline__ bool find_tile(const WinArgs& a, int rows, int t, int
       const int up = __shfl_up(inc, o);
       if (lane >= o) inc += up;
     }
-    const int total = __shfl(inc, 63);
+    const int total = __builtin_amdgcn_readlane(inc, 63);
     if (t < base + total) {
       const int first = __builtin_ctzll(__ballot(base + inc > t));
       seq = s0 + first;
-      tile = __shfl(n, first) - 1 - (t - base - __shfl(inc - n, first));       // latest queries first: they see the most keys
-      seq = __builtin_amdgcn_readfirstlane(seq);
-      tile = __builtin_amdgcn_readfirstlane(tile);
+      tile = __builtin_amdgcn_readlane(n, first) - 1 - (t - base - __builtin_amdgcn_readlane(inc - n, first));     // latest queries first: they see the most keys
       return true;
     }
     base += total;
@@ -384,7 +382,8 @@ template <int QT>
 struct Rows {
   bf16x8 q[QT][4];
   f32x4 o[QT][8];
-  float m[QT], shift[QT], l[QT];       // the maximum that weights are relative to (scaled, log2), minus it (0 while unset), their sum
+  // weights are exp2(scaled score + shift); a sum of them; the largest exponent that is let through: 8, or -inf before the first key
+  float shift[QT], l[QT], lim[QT];
   int pos[QT];
 };
 
@@ -421,58 +420,64 @@ __device__ __forceinline__ void prefill_step(const WinArgs& a, const char* st, i
   const int key = step * 32 + fq * 8;                                  // the lane's scores: keys key .. + 7, of one page
   const bool page = ((fq >> 1) ? pg.p1 : pg.p0) >= 0;
   bf16x8 p[QT];
+  float x[QT][8], mx[QT];
+  bool moves = false;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    float x[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = s[t][0][j];
-      x[j + 4] = s[t][1][j];
-    }
+    for (int j = 0; j < 8; ++j) x[t][j] = fmaf(j < 4 ? s[t][0][j & 3] : s[t][1][j & 3], a.scale_log2, r.shift[t]);
     if (!inside) {
       const int up = page ? r.pos[t] - key : -1, down = r.pos[t] - key - a.window, sink = a.sinks - key;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j <= up && (j > down || j < sink) ? x[j] : -INFINITY;
+      for (int j = 0; j < 8; ++j) x[t][j] = j <= up && (j > down || j < sink) ? x[t][j] : -INFINITY;
     }
-    float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    // The weights are relative to a maximum that is moved only when a score passes it by 8 (a weight of 256): their ratio to
-    // the sum is what counts, and bf16 keeps it at any size. Most steps then need nothing from another lane.
-    if (__ballot(mx * a.scale_log2 > r.m[t] + 8.f) != 0) {
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(r.m[t], mx * a.scale_log2);
-      const float shift = m_new == -INFINITY ? 0.f : -m_new;
-      const float alpha = fast_exp2(r.m[t] + shift);
-      r.m[t] = m_new;
-      r.shift[t] = shift;
+    mx[t] = fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), x[t][2]), x[t][3]), x[t][4]), x[t][5]), x[t][6]), x[t][7]);
+    moves = moves || mx[t] > r.lim[t];
+  }
+  // The maximum that the weights are relative to is moved only when an exponent passes 8 (a weight of 256): the weights' ratio
+  // to their sum is what counts, and bf16 keeps it at any size. Most steps then need nothing from another lane.
+  if (__ballot(moves) != 0) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 16));
+      mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 32));
+      const bool first = r.lim[t] < 0.f, seen = mx[t] > -INFINITY;
+      const float by = first ? (seen ? mx[t] : 0.f) : fmaxf(mx[t], 0.f);
+      const float alpha = first ? 1.f : fast_exp2(-by);
+      r.lim[t] = seen ? 8.f : r.lim[t];
+      r.shift[t] -= by;
       r.l[t] *= alpha;
 #pragma unroll
       for (int n = 0; n < 8; ++n) r.o[t][n] *= alpha;
-    }
-    float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float pj = fast_exp2(fmaf(x[j], a.scale_log2, r.shift[t]));
-      p[t][j] = (__bf16)pj;
-      sum += pj;
+      for (int j = 0; j < 8; ++j) x[t][j] -= by;
     }
-    r.l[t] += sum;
   }
-  const char* vp = st + 8192 + lane * 16;
+  // the sum is taken of the rounded weights, two at a time: they are what meets V
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][j]), (__bf16)fast_exp2(x[t][j + 1])};
+      p[t][j] = two[0];
+      p[t][j + 1] = two[1];
+      r.l[t] = __builtin_amdgcn_fdot2_f32_bf16(two, bf16x2{(__bf16)1.f, (__bf16)1.f}, r.l[t], false);
+    }
+  const char* vp = st + 8192 + (fq >> 1) * 4096 + (lane & 31) * 16;
   // A row that does not see a key has weight 0 for it, and 0 times a NaN or an infinity in V would be NaN: a step at the edge
   // that holds such values sends the wave's rows to careful_tile.
   if (!inside) {
     uint32_t any = 0;
 #pragma unroll 2                                                       // not more: registers
     for (int n = 0; n < 8; ++n) {
-      const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 1024);
+      const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 512);
       any |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
     }
     odd = odd || __ballot(any != 0) != 0;
   }
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 1024);
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 512);
 #pragma unroll
     for (int t = 0; t < QT; ++t) r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
   }
@@ -587,7 +592,8 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
   const int* table = a.tables + (size_t)seq * a.width;
   const int first = ctx - q_len;                                       // position of the sequence's first query
   const unsigned G = a.G, r0 = (unsigned)tile * ROWS;
-  const int tok_a = r0 / G, tb = (r0 + ROWS - 1) / G, tok_b = tb < q_len ? tb : q_len - 1;
+  // (readfirstlane: these are the same in all lanes, and the branches on them are to stay scalar)
+  const int tok_a = __builtin_amdgcn_readfirstlane(r0 / G), tb = __builtin_amdgcn_readfirstlane((r0 + ROWS - 1) / G), tok_b = tb < q_len ? tb : q_len - 1;
   const Span sp = make_span(first + tok_a, first + tok_b, a.window, a.sinks, a.width);
   const int sps = (sp.n + a.splits - 1) / a.splits;
   const int i0 = split * sps, i1 = (i0 + sps) < sp.n ? (i0 + sps) : sp.n;
@@ -600,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     g = R - (unsigned)token * G;
   };
   const unsigned ra = r0 + w * QT * 16;                                // the wave's first and last position; of no rows: nothing is inside
-  const int ta = ra / G, tz = (ra + QT * 16 - 1) / G;
+  const int ta = __builtin_amdgcn_readfirstlane(ra / G), tz = __builtin_amdgcn_readfirstlane((ra + QT * 16 - 1) / G);
   const int pmin = ta < q_len ? first + ta : -1, pmax = first + (tz < q_len ? tz : q_len - 1);
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -618,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     }
 #pragma unroll
     for (int n = 0; n < 8; ++n) r.o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    r.m[t] = -INFINITY;
+    r.lim[t] = -INFINITY;
     r.shift[t] = 0.f;
     r.l[t] = 0.f;
   }
@@ -629,6 +635,9 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     Pages2 pg[RING];
     Stage8 sg;
     const int last = i1 - 1;
+    const int tok = w * 8 + (lane >> 4);
+    const unsigned ko = (tok & 15) * 256 + (((lane & 15) ^ k_key(tok)) << 4);
+    const unsigned vo = ((w & 1) * 64 + (lane >> 5) * 16 + (lane & 15)) * 32 + ((lane >> 4) & 1) * 16;
     if (KV8) {
       pg[0] = pages_of(table, sp.step(i0), a.width, a.pages);
       stage8_load(a, pg[0], h, tid, sg);
@@ -640,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
 #pragma unroll
       for (int j = 0; j < RING - 1; ++j) {
         pg[j] = pages_of(table, sp.step(i0 + j < i1 ? i0 + j : last), a.width, a.pages);
-        dma_step(a, pg[j], h, lds + j * STEP_BYTES, w, lane);
+        dma_step(a, pg[j], h, lds + j * STEP_BYTES, w, ko, vo);
       }
     }
     pg[3] = pages_of(table, sp.step(i0 + 3 < i1 ? i0 + 3 : last), a.width, a.pages);
@@ -657,7 +666,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
         asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        dma_step(a, pg[3], h, lds + ((at + 3) & (RING - 1)) * STEP_BYTES, w, lane);
+        dma_step(a, pg[3], h, lds + ((at + 3) & (RING - 1)) * STEP_BYTES, w, ko, vo);
       }
       const int step = sp.step(i), k0 = step * 32;
       const Pages2 now = pg[0];
@@ -688,7 +697,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     r.l[t] += __shfl_xor(r.l[t], 32);
     int token, g;
     row_of(t, token, g);
-    write_rows(a, token < q_len ? (int64_t)((size_t)(q_start + token) * a.n_q + (size_t)h * G + g) : -1, split, fq, r.o[t], r.m[t], r.l[t]);
+    write_rows(a, token < q_len ? (int64_t)((size_t)(q_start + token) * a.n_q + (size_t)h * G + g) : -1, split, fq, r.o[t], r.lim[t] > 0.f ? -r.shift[t] : -INFINITY, r.l[t]);
   }
 }
 
