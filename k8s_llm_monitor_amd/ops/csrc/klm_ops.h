@@ -186,7 +186,7 @@ int klm_mid_epilogue(const float* part, int ksplit, int M, int N, int kind, void
 // Attention with a sliding window and sinks over the paged cache (llm_window.hip): the token at position p sees key j when
 // j <= p and (j > p - window or j < sinks) and the page table has a page of the cache for it (0 <= id < pages). Decode: `lens` is
 // ctx_lens[n_seqs], q row b stands at position ctx_lens[b] - 1. Prefill: `lens` is seq_info[n_seqs][3] = {q_start, q_len,
-// ctx_len}; rows of no sequence are not written. splits > 1: part_o [rows][n_q][splits][128] and part_ml
+// ctx_len}. splits > 1: part_o [rows][n_q][splits][128] and part_ml
 // [rows][n_q][splits][2] (fp32) are scratch. One struct instead of twenty arguments: a call from Python costs a microsecond less.
 typedef struct klm_window_args {
   const void *q, *k_cache, *v_cache;
@@ -195,6 +195,8 @@ typedef struct klm_window_args {
   float *part_o, *part_ml;
   void* stream;
   int n_seqs, rows, q_stride, n_q, n_kv, width, pages, window, sinks, splits, kv_fp8;
+  int q_tiles;                       // prefill: 16-row query tiles of a wave, 1 or 3
+  int zero_rest;                     // prefill: rows of no sequence become 0 (else they are not written)
   float scale;
 } klm_window_args;
 int klm_window_attn_decode(const klm_window_args* args);

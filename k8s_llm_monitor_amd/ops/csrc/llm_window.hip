@@ -29,6 +29,7 @@ struct WinArgs {
   int width, pages;      // table width, pages in the cache
   int window, sinks;
   int splits;
+  int zero_rest;         // prefill: rows of no sequence become 0
   float scale_log2;
 };
 
@@ -254,30 +255,6 @@ __global__ __launch_bounds__(256) void window_decode_kernel(WinArgs a, int head_
   }
 }
 
-// Joins the splits' parts: one wave per (row, query head), two dims a lane.
-__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, size_t n_heads) {
-  const int lane = threadIdx.x & 63;
-  const size_t head = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (head >= n_heads) return;
-  const float* ml = a.part_ml + head * a.splits * 2;
-  float mt = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) mt = fmaxf(mt, ml[s * 2]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor(mt, o));
-  const float mu = (mt == -INFINITY) ? 0.f : mt;
-  const float2* po = reinterpret_cast<const float2*>(a.part_o + head * a.splits * HD) + lane;
-  float L = 0.f, x = 0.f, y = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float wgt = fast_exp2(ml[s * 2] - mu);
-    const float2 v = po[s * (HD / 2)];
-    L += ml[s * 2 + 1] * wgt;
-    x += v.x * wgt;
-    y += v.y * wgt;
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  reinterpret_cast<uint32_t*>(a.out + head * HD)[lane] = (uint32_t)f2bf(x * inv) | ((uint32_t)f2bf(y * inv) << 16);
-}
-
 // ---------------------------------------------------------------------------------------------------------------------
 // Prompts and chunks of prompts. Query rows are (token, head of the kv head's group) pairs in a row; a wave takes QT tiles of
 // 16 of them, a block of 4 waves walks the 32-key steps they may see, staged through LDS as bf16. The operand mapping is
@@ -288,60 +265,69 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a, size_t n_he
 // brought in by LDS-DMA three steps ahead (4 KiB a wave, no registers), an e4m3 cache through registers, where it becomes
 // bf16 once per block.
 // ---------------------------------------------------------------------------------------------------------------------
-#ifndef QTILES
-#define QTILES 3
-#endif
 constexpr int STEP_BYTES = 16384, RING = 4;
 
 __device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) & 3) << 2); }
 
-#define KLM_AS1 __attribute__((address_space(1)))
 #define KLM_AS3 __attribute__((address_space(3)))
-#define KLM_AS4 __attribute__((address_space(4)))
 struct Pages2 {
   int p0, p1;            // a step's two pages, -1: none
 };
-// Through the scalar cache: the index is the same in all lanes, and the vector memory counter stays with the DMA. A step of a
-// span has its first page inside the table.
-__device__ __forceinline__ Pages2 pages_of(const int* table, int step, int width, int pages) {
-  const KLM_AS4 int* t = (const KLM_AS4 int*)table;
-  const int i1 = step * 2 + 1 < width ? step * 2 + 1 : width - 1;
-  const int a = t[step * 2], b = t[i1];
-  return Pages2{(unsigned)a < (unsigned)pages ? a : -1, (unsigned)b < (unsigned)pages && step * 2 + 1 < width ? b : -1};
-}
 
 // A wave brings a quarter of a step, half a page: K tokens 8w .. 8w + 7 (the chunk swizzle is the same for both fours of
 // them), V dims 64 (w % 2) .. + 63; `ko`, `vo`: the lane's offsets in bytes inside the page. The second half of each lies 1 KiB
 // behind the first, in memory as in LDS.
-__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, char* st, int w, unsigned ko, unsigned vo) {
+// Written in assembly because the compiler takes the builtin for an access that may hit LDS at any time, and then waits for all
+// outstanding LDS reads at each of them (and for the DMA before them); what has landed is said by the kernel's own waits. No
+// register is written but m0, which nothing else here uses. s_nop 4: a scalar base that a vector instruction wrote may be
+// read by a memory instruction five states later; s_nop 0: m0 before its use.
+__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, uint32_t st, int w, unsigned ko, unsigned vo) {
   const int id = w < 2 ? pg.p0 : pg.p1;
   const size_t base = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * (BLK_ELEMS * 2);
   const char* k = (const char*)a.kc + base;
   const char* v = (const char*)a.vc + base;
-  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(k + ko), (KLM_AS3 void*)(st + w * 2048), 16, 0, 0);
-  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(k + ko), (KLM_AS3 void*)(st + w * 2048), 16, 1024, 0);
-  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(v + vo), (KLM_AS3 void*)(st + 8192 + w * 2048), 16, 0, 0);
-  __builtin_amdgcn_global_load_lds((const KLM_AS1 void*)(v + vo), (KLM_AS3 void*)(st + 8192 + w * 2048), 16, 1024, 0);
+  asm volatile(
+      "s_mov_b32 m0, %4\n\t"
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %0, %2\n\t"
+      "global_load_lds_dwordx4 %0, %2 offset:1024\n\t"
+      "s_mov_b32 m0, %5\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %3\n\t"
+      "global_load_lds_dwordx4 %1, %3 offset:1024"
+      :
+      : "v"(ko), "v"(vo), "s"(k), "s"(v), "s"(st + w * 2048), "s"(st + 8192 + w * 2048)
+      : "memory");
 }
 
-struct Stage8 {
-  uint4 k, v;
-};
-__device__ __forceinline__ void stage8_load(const WinArgs& a, Pages2 pg, int h, int tid, Stage8& s) {
-  const int id = (tid >> 7) ? pg.p1 : pg.p0;
-  const size_t o = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * BLK_ELEMS + (tid & 127) * 16;
-  s.k = *reinterpret_cast<const uint4*>((const uint8_t*)a.kc + o);
-  s.v = *reinterpret_cast<const uint4*>((const uint8_t*)a.vc + o);
+// The same of an e4m3 cache: a wave's 2 KiB of raw bytes go to a corner of its own, `raw`, from where it turns them into the bf16
+// step one step later. A lane's 16 bytes: 16 dims of a key, 16 tokens of a dim.
+__device__ __forceinline__ void dma_step8(const WinArgs& a, Pages2 pg, int h, uint32_t raw, int w, unsigned off) {
+  const int id = w < 2 ? pg.p0 : pg.p1;
+  const size_t base = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * BLK_ELEMS + (w & 1) * 1024;
+  const char* k = (const char*)a.kc + base;
+  const char* v = (const char*)a.vc + base;
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %0, %1\n\t"
+      "s_mov_b32 m0, %4\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %0, %2"
+      :
+      : "v"(off), "s"(k), "s"(v), "s"(raw), "s"(raw + 1024)
+      : "memory");
 }
-__device__ __forceinline__ void stage8_store(char* st, int tid, const Stage8& s) {
-  const int tok = tid >> 3, c = (tid & 7) * 2, key = k_key(tok);
+__device__ __forceinline__ void widen_step8(char* st, const char* raw, int w, int lane) {
+  const uint4 k = *reinterpret_cast<const uint4*>(raw + lane * 16), v = *reinterpret_cast<const uint4*>(raw + 1024 + lane * 16);
+  const int tok = w * 8 + (lane >> 3), c = (lane & 7) * 2, key = k_key(tok);
   char* kp = st + tok * 256;
-  *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(s.k.x, s.k.y);
-  *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(s.k.z, s.k.w);
-  const int page = tid >> 7, dim = tid & 127;
-  char* vp = st + 8192 + page * 4096 + (dim >> 4) * 512 + (dim & 15) * 16;
-  *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(s.v.x, s.v.y);
-  *reinterpret_cast<bf16x8*>(vp + 256) = fp8x8_to_bf16(s.v.z, s.v.w);
+  *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(k.x, k.y);
+  *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(k.z, k.w);
+  const int dim = (w & 1) * 64 + lane;
+  char* vp = st + 8192 + (w >> 1) * 4096 + (dim >> 4) * 512 + (dim & 15) * 16;
+  *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(v.x, v.y);
+  *reinterpret_cast<bf16x8*>(vp + 256) = fp8x8_to_bf16(v.z, v.w);
 }
 
 // a row of seq_info that counts: queries inside q, and a context that holds them (rows * G fits 31 bits, see the launcher)
@@ -349,32 +335,50 @@ __device__ __forceinline__ bool is_sequence(const WinArgs& a, int q_start, int q
   return q_len > 0 && ctx >= q_len && q_start >= 0 && q_len <= a.rows && q_start <= a.rows - q_len;
 }
 
-// tile t of the launch -> its sequence and its number among the sequence's tiles; false: the launch has more tiles than needed
-__device__ __forceinline__ bool find_tile(const WinArgs& a, int rows, int t, int lane, int& seq, int& tile) {
+// Tile t of the launch -> its sequence and its number among the sequence's tiles (seq < 0: the launch has more tiles than
+// needed), and how many rows the sequences have together.
+__device__ __forceinline__ void find_tile(const WinArgs& a, int rows, int t, int lane, int& seq, int& tile, int& in_use) {
   int base = 0;
+  seq = -1;
+  tile = 0;
+  in_use = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
     const int i = s0 + lane;
-    int n = 0;
+    int n = 0, m = 0;
     if (i < a.n_seqs) {
       const int qs = a.lens[i * 3], ql = a.lens[i * 3 + 1], cl = a.lens[i * 3 + 2];
-      if (is_sequence(a, qs, ql, cl)) n = (int)(((unsigned)(ql * a.G) + rows - 1) / rows);
+      if (is_sequence(a, qs, ql, cl)) {
+        n = (int)(((unsigned)(ql * a.G) + rows - 1) / rows);
+        m = ql;
+      }
     }
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int up = __shfl_up(inc, o);
       if (lane >= o) inc += up;
+      if (a.zero_rest) m += __shfl_xor(m, o);
     }
+    in_use += __builtin_amdgcn_readfirstlane(m);
     const int total = __builtin_amdgcn_readlane(inc, 63);
-    if (t < base + total) {
+    if (seq < 0 && t < base + total) {
       const int first = __builtin_ctzll(__ballot(base + inc > t));
       seq = s0 + first;
       tile = __builtin_amdgcn_readlane(n, first) - 1 - (t - base - __builtin_amdgcn_readlane(inc - n, first));     // latest queries first: they see the most keys
-      return true;
+      if (!a.zero_rest) return;
     }
     base += total;
   }
-  return false;
+}
+
+// Is `row` one of a sequence's?
+__device__ __forceinline__ bool owned(const WinArgs& a, int row, int lane) {
+  bool mine = false;
+  for (int i = lane; i < a.n_seqs; i += 64) {
+    const int qs = a.lens[i * 3], ql = a.lens[i * 3 + 1];
+    mine = mine || (is_sequence(a, qs, ql, a.lens[i * 3 + 2]) && row >= qs && row < qs + ql);
+  }
+  return __ballot(mine) != 0;
 }
 
 // A wave's state: QT tiles of 16 query rows, lane (fr, fq) has row fr of each.
@@ -399,88 +403,106 @@ __device__ __forceinline__ uint32_t odd_marks(uint32_t x) {
   return r;
 }
 
-// One 32-key step for the wave's rows. inside (wave-uniform): every row in use sees every key of the step.
+// What a wave does with one 32-key step, in two parts, so that matrix and vector instructions of different steps can run at the
+// same time: while the scores of step i + 1 are multiplied, the weights of step i are taken from their exponents (part A); while
+// step i's weights meet V, step i + 1's scores become exponents (part B).
 template <int QT>
-__device__ __forceinline__ void prefill_step(const WinArgs& a, const char* st, int step, Pages2 pg, bool inside, int lane, Rows<QT>& r, bool& odd) {
+struct Scores {
+  f32x4 s[QT][2];
+};
+
+template <int QT>
+__device__ __forceinline__ void part_a(const char* st, int lane, Rows<QT>& r, const float (&x)[QT][8], Scores<QT>& s, bf16x8 (&p)[QT]) {
   const int fr = lane & 15, fq = lane >> 4;
   const char* kp = st + ((fr >> 2) * 8 + (fr & 3)) * 256;              // k_key of both tokens below is fr
-  f32x4 s[QT][2];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < QT; ++t) s.s[t][0] = s.s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
     const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s[t][0], 0, 0, 0);
-      s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s[t][1], 0, 0, 0);
-    }
-  }
-  const int key = step * 32 + fq * 8;                                  // the lane's scores: keys key .. + 7, of one page
-  const bool page = ((fq >> 1) ? pg.p1 : pg.p0) >= 0;
-  bf16x8 p[QT];
-  float x[QT][8], mx[QT];
-  bool moves = false;
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[t][j] = fmaf(j < 4 ? s[t][0][j & 3] : s[t][1][j & 3], a.scale_log2, r.shift[t]);
-    if (!inside) {
-      const int up = page ? r.pos[t] - key : -1, down = r.pos[t] - key - a.window, sink = a.sinks - key;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[t][j] = j <= up && (j > down || j < sink) ? x[t][j] : -INFINITY;
-    }
-    mx[t] = fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), x[t][2]), x[t][3]), x[t][4]), x[t][5]), x[t][6]), x[t][7]);
-    moves = moves || mx[t] > r.lim[t];
-  }
-  // The maximum that the weights are relative to is moved only when an exponent passes 8 (a weight of 256): the weights' ratio
-  // to their sum is what counts, and bf16 keeps it at any size. Most steps then need nothing from another lane.
-  if (__ballot(moves) != 0) {
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 16));
-      mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 32));
-      const bool first = r.lim[t] < 0.f, seen = mx[t] > -INFINITY;
-      const float by = first ? (seen ? mx[t] : 0.f) : fmaxf(mx[t], 0.f);
-      const float alpha = first ? 1.f : fast_exp2(-by);
-      r.lim[t] = seen ? 8.f : r.lim[t];
-      r.shift[t] -= by;
-      r.l[t] *= alpha;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) r.o[t][n] *= alpha;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[t][j] -= by;
-    }
-  }
-  // the sum is taken of the rounded weights, two at a time: they are what meets V
-#pragma unroll
-  for (int t = 0; t < QT; ++t)
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][j]), (__bf16)fast_exp2(x[t][j + 1])};
-      p[t][j] = two[0];
-      p[t][j + 1] = two[1];
+      s.s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s.s[t][0], 0, 0, 0);
+      s.s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s.s[t][1], 0, 0, 0);
+      // the sum is taken of the rounded weights, two at a time: they are what meets V
+      const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][2 * c]), (__bf16)fast_exp2(x[t][2 * c + 1])};
+      p[t][2 * c] = two[0];
+      p[t][2 * c + 1] = two[1];
       r.l[t] = __builtin_amdgcn_fdot2_f32_bf16(two, bf16x2{(__bf16)1.f, (__bf16)1.f}, r.l[t], false);
     }
-  const char* vp = st + 8192 + (fq >> 1) * 4096 + (lane & 31) * 16;
-  // A row that does not see a key has weight 0 for it, and 0 times a NaN or an infinity in V would be NaN: a step at the edge
-  // that holds such values sends the wave's rows to careful_tile.
-  if (!inside) {
-    uint32_t any = 0;
-#pragma unroll 2                                                       // not more: registers
-    for (int n = 0; n < 8; ++n) {
-      const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 512);
-      any |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
-    }
-    odd = odd || __ballot(any != 0) != 0;
   }
+}
+
+template <int QT>
+__device__ __forceinline__ void part_b(const WinArgs& a, const char* st, int lane, Rows<QT>& r, const Scores<QT>& s, const bf16x8 (&p)[QT],
+                                       float (&x)[QT][8], float (&mx)[QT]) {
+  const int fq = lane >> 4;
+  const char* vp = st + 8192 + (fq >> 1) * 4096 + (lane & 31) * 16;
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
     const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 512);
 #pragma unroll
-    for (int t = 0; t < QT; ++t) r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
+    for (int t = 0; t < QT; ++t) {
+      r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
+      x[t][n] = fmaf(n < 4 ? s.s[t][0][n & 3] : s.s[t][1][n & 3], a.scale_log2, r.shift[t]);
+      mx[t] = n ? fmaxf(mx[t], x[t][n]) : x[t][n];
+    }
   }
+}
+
+// Masks the exponents of a step that some row does not see whole.
+template <int QT>
+__device__ __forceinline__ void mask_step(const WinArgs& a, int step, Pages2 pg, int lane, const Rows<QT>& r, float (&x)[QT][8], float (&mx)[QT]) {
+  const int fq = lane >> 4, key = step * 32 + fq * 8;                  // the lane's scores: keys key .. + 7, of one page
+  const bool page = ((fq >> 1) ? pg.p1 : pg.p0) >= 0;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int up = page ? r.pos[t] - key : -1, down = r.pos[t] - key - a.window, sink = a.sinks - key;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[t][j] = j <= up && (j > down || j < sink) ? x[t][j] : -INFINITY;
+      mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
+    }
+  }
+}
+
+// The maximum that the weights are relative to is moved only when an exponent passes 8 (a weight of 256): the weights' ratio to
+// their sum is what counts, and bf16 keeps it at any size. Most steps then need nothing from another lane.
+template <int QT>
+__device__ __forceinline__ void move_maximum(Rows<QT>& r, float (&x)[QT][8], float (&mx)[QT]) {
+  bool moves = false;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) moves = moves || mx[t] > r.lim[t];
+  if (__ballot(moves) == 0) return;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 16));
+    mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 32));
+    const bool first = r.lim[t] < 0.f, seen = mx[t] > -INFINITY;
+    const float by = first ? (seen ? mx[t] : 0.f) : fmaxf(mx[t], 0.f);
+    const float alpha = first ? 1.f : fast_exp2(-by);
+    r.lim[t] = seen ? 8.f : r.lim[t];
+    r.shift[t] -= by;
+    r.l[t] *= alpha;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) r.o[t][n] *= alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[t][j] -= by;
+  }
+}
+
+// A row that does not see a key has weight 0 for it, and 0 times a NaN or an infinity in V would be NaN: a step at the edge that
+// holds such values sends the wave's rows to careful_tile.
+__device__ __forceinline__ bool odd_values(const char* st, int lane) {
+  const char* vp = st + 8192 + lane * 16;
+  uint32_t any = 0;
+#pragma unroll 2                                                       // not more: registers
+  for (int n = 0; n < 8; ++n) {
+    const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 1024);
+    any |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
+  }
+  return __ballot(any != 0) != 0;
 }
 
 // The finished rows of one 16-row tile: lane (fr, fq) holds dims n * 16 + fq * 4 .. + 3 of row fr; dst < 0: no row.
@@ -586,8 +608,16 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   constexpr int ROWS = 64 * QT;
-  int seq, tile;
-  if (!find_tile(a, ROWS, blockIdx.y, lane, seq, tile)) return;
+  int seq, tile, in_use;
+  find_tile(a, ROWS, blockIdx.y, lane, seq, tile, in_use);
+  if (a.zero_rest && a.splits == 1 && in_use < a.rows) {               // this block's share of the rows that may be nobody's
+    const int share = (a.rows + gridDim.y - 1) / gridDim.y;
+    for (int row = blockIdx.y * share + w; row < a.rows && row < (int)(blockIdx.y + 1) * share; row += 4)
+      if (!owned(a, row, lane))
+        for (int e = lane * 8; e < a.G * HD; e += 512)
+          *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.n_q + (size_t)h * a.G) * HD + e) = uint4{0, 0, 0, 0};
+  }
+  if (seq < 0) return;
   const int q_start = a.lens[seq * 3], q_len = a.lens[seq * 3 + 1], ctx = a.lens[seq * 3 + 2];
   const int* table = a.tables + (size_t)seq * a.width;
   const int first = ctx - q_len;                                       // position of the sequence's first query
@@ -631,50 +661,112 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
 
   bool odd = false;
   if (i0 < i1) {
-    // pages of the step that is computed, and of the steps that are on their way
-    Pages2 pg[RING];
-    Stage8 sg;
     const int last = i1 - 1;
     const int tok = w * 8 + (lane >> 4);
     const unsigned ko = (tok & 15) * 256 + (((lane & 15) ^ k_key(tok)) << 4);
     const unsigned vo = ((w & 1) * 64 + (lane >> 5) * 16 + (lane & 15)) * 32 + ((lane >> 4) & 1) * 16;
+    const auto step_of = [&](int i) { return sp.step(i < last ? i : last); };      // past the last step: that one again, unused
+    const auto is_inside = [&](int step, Pages2 pg) {
+      const int k0 = step * 32;
+      return k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && pg.p0 >= 0 && pg.p1 >= 0;
+    };
+    // Pages of step i + 1, i + 2 and i + 3. At step i its V and the K of i + 1 are in LDS, i + 2 is on its way, and i + 3 takes the
+    // place of i - 1, which all waves have left at the barrier.
+    // The table's entries for 32 steps at a time lie in one register, a lane each: looking them up in the loop through the scalar
+    // cache would share the LDS reads' counter and make every wait on them a wait for all of them.
+    int held;
+    const auto hold = [&](int i) {                                     // steps i .. i + 31
+      const int e = step_of(i + (lane >> 1)) * 2 + (lane & 1);
+      const int id = table[e < a.width ? e : a.width - 1];
+      held = e < a.width && (unsigned)id < (unsigned)a.pages ? id : -1;
+    };
+    const auto pages_at = [&](int i) {                                 // of step i0 + i, i in the 32 that are held
+      return Pages2{__builtin_amdgcn_readlane(held, (i & 31) * 2), __builtin_amdgcn_readlane(held, (i & 31) * 2 + 1)};
+    };
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((KLM_AS3 char*)lds);
+    hold(i0);
+    const Pages2 now = pages_at(0);
+    Pages2 next = pages_at(1), after = pages_at(2), far = pages_at(3);
+    // e4m3: two raw corners a wave behind the ring. Step i + 2 is widened at step i, while i + 3 lands in the other corner.
+    const uint32_t raw0 = lds0 + RING * STEP_BYTES + w * 2048;
+    char* const raws = lds + RING * STEP_BYTES + w * 2048;
+    const unsigned off = lane * 16;
     if (KV8) {
-      pg[0] = pages_of(table, sp.step(i0), a.width, a.pages);
-      stage8_load(a, pg[0], h, tid, sg);
-      stage8_store(lds, tid, sg);
-      pg[1] = pages_of(table, sp.step(i0 + 1 < i1 ? i0 + 1 : last), a.width, a.pages);
-      stage8_load(a, pg[1], h, tid, sg);
-      pg[2] = pages_of(table, sp.step(i0 + 2 < i1 ? i0 + 2 : last), a.width, a.pages);
+      dma_step8(a, now, h, raw0, w, off);
+      dma_step8(a, next, h, raw0 + 8192, w, off);
+      asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+      widen_step8(lds, raws, w, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the corner has been read
+      dma_step8(a, after, h, raw0, w, off);
+      asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+      widen_step8(lds + STEP_BYTES, raws + 8192, w, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
-#pragma unroll
-      for (int j = 0; j < RING - 1; ++j) {
-        pg[j] = pages_of(table, sp.step(i0 + j < i1 ? i0 + j : last), a.width, a.pages);
-        dma_step(a, pg[j], h, lds + j * STEP_BYTES, w, ko, vo);
-      }
+      dma_step(a, now, h, lds0, w, ko, vo);
+      dma_step(a, next, h, lds0 + STEP_BYTES, w, ko, vo);
+      dma_step(a, after, h, lds0 + 2 * STEP_BYTES, w, ko, vo);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     }
-    pg[3] = pages_of(table, sp.step(i0 + 3 < i1 ? i0 + 3 : last), a.width, a.pages);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    float x[QT][8], mx[QT];
+    bf16x8 p[QT];
+    bool inside = is_inside(sp.step(i0), now);
+    {
+      Scores<QT> s;
+      const char* kp = lds + ((fr >> 2) * 8 + (fr & 3)) * 256;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) s.s[t][0] = s.s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
+        const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          s.s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s.s[t][0], 0, 0, 0);
+          s.s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s.s[t][1], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[t][j] = (j < 4 ? s.s[t][0][j & 3] : s.s[t][1][j & 3]) * a.scale_log2;
+          mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
+        }
+    }
+    if (!inside) mask_step<QT>(a, sp.step(i0), now, lane, r, x, mx);
+    move_maximum<QT>(r, x, mx);
     for (int i = i0; i < i1; ++i) {
       const int at = i - i0;
       if (KV8) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             // this wave's part of step i is in LDS
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the raw step i + 2 has landed, this wave's part of i + 1 is written
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        stage8_store(lds + ((at + 1) & (RING - 1)) * STEP_BYTES, tid, sg);
-        stage8_load(a, pg[2], h, tid, sg);
+        dma_step8(a, far, h, raw0 + ((at + 1) & 1) * 8192, w, off);    // read for the last time one step ago
+        widen_step8(lds + ((at + 2) & (RING - 1)) * STEP_BYTES, raws + (at & 1) * 8192, w, lane);
       } else {
-        // 4 DMA instructions a wave and step, in order: at most those of the two newer steps may be on their way
-        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");               // 4 DMA instructions a wave and step, in order: i + 1 has landed
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        dma_step(a, pg[3], h, lds + ((at + 3) & (RING - 1)) * STEP_BYTES, w, ko, vo);
+        dma_step(a, far, h, lds0 + ((at + 3) & (RING - 1)) * STEP_BYTES, w, ko, vo);
       }
-      const int step = sp.step(i), k0 = step * 32;
-      const Pages2 now = pg[0];
-      pg[0] = pg[1]; pg[1] = pg[2]; pg[2] = pg[3];
-      pg[3] = pages_of(table, sp.step(i + 4 < i1 ? i + 4 : last), a.width, a.pages);
       const char* st = lds + (at & (RING - 1)) * STEP_BYTES;
-      const bool inside = k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && now.p0 >= 0 && now.p1 >= 0;
-      prefill_step<QT>(a, st, step, now, inside, lane, r, odd);
+      const char* st1 = lds + ((at + 1) & (RING - 1)) * STEP_BYTES;
+      const int step1 = step_of(i + 1);
+      const bool inside1 = is_inside(step1, next);
+      const Pages2 pg1 = next;
+      next = after;
+      after = far;
+      if (((at + 4) & 31) == 0) hold(i + 4);
+      far = pages_at(at + 4);
+      if (!inside) odd = odd || odd_values(st, lane);
+      Scores<QT> s;
+      part_a<QT>(st1, lane, r, x, s, p);
+      part_b<QT>(a, st, lane, r, s, p, x, mx);
+      if (!inside1) mask_step<QT>(a, step1, pg1, lane, r, x, mx);
+      move_maximum<QT>(r, x, mx);
+      inside = inside1;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // the last, unused steps land before the LDS goes away
   }
@@ -701,6 +793,38 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
   }
 }
 
+// Joins the splits' parts: one wave per (row, query head), two dims a lane.
+template <bool PREFILL>
+__global__ __launch_bounds__(256) void window_join_kernel(WinArgs a) {
+  const int lane = threadIdx.x & 63, row = blockIdx.y;
+  const int h = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (h >= a.n_q) return;
+  const size_t head = (size_t)row * a.n_q + h;
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.out + head * HD) + lane;
+  if (PREFILL && !owned(a, row, lane)) {                               // its parts were not written
+    if (a.zero_rest) *out = 0;
+    return;
+  }
+  const float* ml = a.part_ml + head * a.splits * 2;
+  float mt = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) mt = fmaxf(mt, ml[s * 2]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor(mt, o));
+  const float mu = (mt == -INFINITY) ? 0.f : mt;
+  const float2* po = reinterpret_cast<const float2*>(a.part_o + head * a.splits * HD) + lane;
+  float L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float wgt = fast_exp2(ml[s * 2] - mu);
+    const float2 v = po[s * (HD / 2)];
+    L += ml[s * 2 + 1] * wgt;
+    x += v.x * wgt;
+    y += v.y * wgt;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *out = (uint32_t)f2bf(x * inv) | ((uint32_t)f2bf(y * inv) << 16);
+}
+
 int check_args(const WinArgs& a) {
   if (a.rows <= 0 || a.n_seqs <= 0 || a.n_seqs > 65535 || a.n_q <= 0 || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.width <= 0 || a.pages <= 0 ||
       a.q_stride < a.n_q * HD || a.q_stride % 8 != 0 || a.width > INT32_MAX / BLK - 2)
@@ -715,7 +839,24 @@ int check_args(const WinArgs& a) {
 WinArgs device_args(const klm_window_args* c) {
   return WinArgs{(const uint16_t*)c->q, c->k_cache, c->v_cache, c->tables, c->lens, (uint16_t*)c->out, c->part_o, c->part_ml,
                  c->n_seqs, c->rows, c->q_stride, c->n_q, c->n_kv, c->n_kv > 0 ? c->n_q / c->n_kv : 0, c->width, c->pages,
-                 c->window, c->sinks, c->splits, c->scale * 1.4426950408889634f};
+                 c->window, c->sinks, c->splits, c->zero_rest, c->scale * 1.4426950408889634f};
+}
+
+template <bool PREFILL>
+int launch_join(const WinArgs& a, hipStream_t s) {
+  if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
+  if (a.splits > 1) hipLaunchKernelGGL(window_join_kernel<PREFILL>, dim3((a.n_q + 3) / 4, a.rows), dim3(256), 0, s, a);
+  return launch_status();
+}
+
+template <int QT, bool KV8>
+int launch_prefill(const WinArgs& a, hipStream_t s) {
+  constexpr int LDS = RING * STEP_BYTES + (KV8 ? 16384 : 0);
+  const int64_t tiles = ((int64_t)a.rows * a.G + 64 * QT - 1) / (64 * QT) + a.n_seqs;       // every sequence may end in a partial tile
+  if (tiles > 65535 || (int64_t)a.rows * a.G > (1 << 30) || (a.splits > 1 && a.rows > 65535)) return KLM_ERR_SHAPE;
+  if (klm_ensure_dyn_lds<window_prefill_kernel<QT, KV8>>(LDS) != KLM_OK) return KLM_ERR_HIP;
+  hipLaunchKernelGGL((window_prefill_kernel<QT, KV8>), dim3(a.n_kv, (unsigned)tiles, a.splits), dim3(256), LDS, s, a);
+  return launch_join<true>(a, s);
 }
 
 }  // namespace
@@ -733,12 +874,7 @@ int klm_window_attn_decode(const klm_window_args* c) {
   const dim3 grid(a.n_kv * head_tiles, a.rows, a.splits);
   if (c->kv_fp8) hipLaunchKernelGGL(window_decode_kernel<true>, grid, dim3(256), 0, s, a, head_tiles);
   else hipLaunchKernelGGL(window_decode_kernel<false>, grid, dim3(256), 0, s, a, head_tiles);
-  if (hipGetLastError() != hipSuccess) return KLM_ERR_HIP;
-  if (a.splits > 1) {
-    const size_t heads = (size_t)a.rows * a.n_q;
-    hipLaunchKernelGGL(window_join_kernel, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a, heads);
-  }
-  return launch_status();
+  return launch_join<false>(a, s);
 }
 
 int klm_window_attn_prefill(const klm_window_args* c) {
@@ -746,13 +882,12 @@ int klm_window_attn_prefill(const klm_window_args* c) {
   const WinArgs a = device_args(c);
   const int rc = check_args(a);
   if (rc != KLM_OK) return rc;
-  const int64_t tiles = ((int64_t)a.rows * a.G + 64 * QTILES - 1) / (64 * QTILES) + a.n_seqs;       // every sequence may end in a partial tile
-  if (tiles > 65535 || (int64_t)a.rows * a.G > (1 << 30)) return KLM_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(c->stream);
-  const dim3 grid(a.n_kv, (unsigned)tiles, 1);
-  if (c->kv_fp8) hipLaunchKernelGGL((window_prefill_kernel<QTILES, true>), grid, dim3(256), RING * STEP_BYTES, s, a);
-  else hipLaunchKernelGGL((window_prefill_kernel<QTILES, false>), grid, dim3(256), RING * STEP_BYTES, s, a);
-  return launch_status();
+  switch (c->q_tiles) {
+    case 1: return c->kv_fp8 ? launch_prefill<1, true>(a, s) : launch_prefill<1, false>(a, s);
+    case 3: return c->kv_fp8 ? launch_prefill<3, true>(a, s) : launch_prefill<3, false>(a, s);
+    default: return KLM_ERR_VARIANT;
+  }
 }
 
 }  // extern "C"

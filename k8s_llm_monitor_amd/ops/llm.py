@@ -610,7 +610,7 @@ def paged_attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
 # ------------------------------------------------------------------ sliding window and sinks
 _FAR = 1 << 30          # a window or sinks beyond any context; keeps the kernels' 32-bit positions from running over
-_WINDOW_ARGS = struct.Struct("9P11if")          # klm_window_args
+_WINDOW_ARGS = struct.Struct("9P13if")          # klm_window_args
 
 
 def _call(fn, args: bytes, t: torch.Tensor) -> int:
@@ -688,10 +688,18 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     rc = _call(_lib().klm_window_attn_decode,
                _WINDOW_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), ctx_lens.data_ptr(),
                                  out.data_ptr(), part_o, part_ml, _stream(q), B, B, q.stride(0) if B > 1 else n_q * HEAD_DIM, n_q, n_kv,
-                                 width, nb, window, sinks, splits, _kv8(k_cache), scale), q)
+                                 width, nb, window, sinks, splits, _kv8(k_cache), 0, 0, scale), q)
     if rc:
         _check(rc, f"klm_window_attn_decode(B={B},window={window},sinks={sinks},splits={splits})")
     return out
+
+
+def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int) -> Tuple[int, int]:
+    """(16-row tiles a wave, splits of the keys) of `paged_attn_prefill_window`, `reach` keys being the most that a query sees."""
+    if (rows * group // 192 + seqs) * n_kv >= 256:
+        return 3, 1
+    blocks = (-(-rows * group // 64) + seqs - 1) * n_kv
+    return 1, max(1, min(512 // blocks, (reach // 32 + 1) // 4, 32))
 
 
 def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -713,14 +721,22 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         raise KlmOpsError(f"{what}: seq_info {tuple(seq_info.shape)} for {S} table rows")
     if not q.is_cuda:
         return ref.window_attn_prefill(q[:, : n_q * HEAD_DIM], k_cache, v_cache, block_tables, seq_info, scale, window, sinks, out)
-    if out is None:
-        out = q.new_zeros((T, n_q * HEAD_DIM))
+    zero_rest = out is None
     if T == 0 or S == 0:
-        return out
+        return q.new_zeros((T, n_q * HEAD_DIM)) if zero_rest else out
+    if zero_rest:
+        out = q.new_empty((T, n_q * HEAD_DIM))
+    window, sinks = min(window, _FAR), min(sinks, _FAR)
+    q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK))
+    part_o = part_ml = 0
+    if splits > 1:
+        scratch = torch.empty(T * n_q * splits * (HEAD_DIM + 2), dtype=torch.float32, device=q.device)
+        part_o = scratch.data_ptr()
+        part_ml = part_o + T * n_q * splits * HEAD_DIM * 4
     rc = _call(_lib().klm_window_attn_prefill,
                _WINDOW_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_info.data_ptr(),
-                                 out.data_ptr(), 0, 0, _stream(q), S, T, q.stride(0) if T > 1 else n_q * HEAD_DIM, n_q, n_kv, width, nb,
-                                 min(window, _FAR), min(sinks, _FAR), 1, _kv8(k_cache), scale), q)
+                                 out.data_ptr(), part_o, part_ml, _stream(q), S, T, q.stride(0) if T > 1 else n_q * HEAD_DIM, n_q, n_kv, width, nb,
+                                 window, sinks, splits, _kv8(k_cache), q_tiles, zero_rest, scale), q)
     if rc:
         _check(rc, f"klm_window_attn_prefill(T={T},S={S},window={window},sinks={sinks})")
     return out

@@ -179,6 +179,38 @@ def test_strides_given_out_and_untouched_rows():
         _decode(wide[:, 63:63 + 1024], k, v, table, lens, 8, 30, 2)       # 2-byte alignment
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("seqs,rows,n_q,n_kv", [([(5, 20, 3000)], 40, 8, 2), ([(0, 3, 2000), (7, 9, 10), (30, 2, 1)], 33, 4, 4), ([(9, 2000, 2100), (2010, 1, 1)], 2020, 32, 8)])
+def test_rows_of_no_sequence_whatever_the_launch(dtype, seqs, rows, n_q, n_kv):
+    """Few rows (split keys and their join), many rows (one pass): rows that no sequence has are 0, or as they were in a given out."""
+    q, k, v, table = _random("prefill", seqs, n_q, n_kv, dtype)
+    q = torch.cat([q, torch.randn(rows - q.shape[0], q.shape[1], device=DEV).to(torch.bfloat16)])
+    mine = torch.zeros(rows, dtype=torch.bool)
+    for q0, ql, n in seqs:
+        mine[q0:q0 + ql] |= n >= ql
+    want, size = _reference("prefill", q, k, v, table, seqs, 1900, 5)
+    fresh = _prefill(q, k, v, table, seqs, n_q, 1900, 5)
+    _near(fresh, want, size)
+    assert not fresh[~mine].any()
+    given = torch.full_like(fresh, 3.0)
+    _prefill(q, k, v, table, seqs, n_q, 1900, 5, out=given)
+    assert torch.equal(given[mine], fresh[mine]) and (given[~mine] == 3).all()
+
+
+def test_rows_of_seq_info_that_are_no_sequences():
+    """Queries that do not lie in q, a context shorter than the queries, negative numbers: skipped, their rows are nobody's."""
+    good = (4, 6, 30)
+    for bad in ((-1, 3, 10), (20, 5, 9), (0, 40, 50), (0, 3, 2), (0, -2, 5), (0, 3, -3), (2 ** 31 - 1, 3, 9), (0, 2 ** 31 - 1, 2 ** 31 - 1)):
+        q, k, v, table = make("prefill", [good, (10, 2, 5)], 4, 2, 9, 2, spare=10)
+        info = torch.tensor([good, bad], dtype=torch.int32, device=DEV)
+        a = [x.to(DEV) for x in (q, k, v, table)]
+        got = llm.paged_attn_prefill_window(*a, info, SCALE, 4, 9, 2)
+        want = llm.paged_attn_prefill_window(a[0], a[1], a[2], a[3][:1].contiguous(), info[:1].contiguous(), SCALE, 4, 9, 2)
+        assert torch.equal(got, want) and got[4:10].any() and not got[:4].any() and not got[10:].any()
+        cpu = llm.paged_attn_prefill_window(q.float(), k.float(), v.float(), table, info.cpu(), SCALE, 4, 9, 2)
+        assert torch.equal(cpu.any(1), got.cpu().any(1))
+
+
 def test_refusals_on_the_gpu():
     q, k, v, table = (x.to(DEV) for x in make("decode", [20, 3], 4, 2, 8, 0))
     lens = torch.tensor([20, 3], dtype=torch.int32, device=DEV)
