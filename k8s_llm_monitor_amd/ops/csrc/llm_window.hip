@@ -371,7 +371,7 @@ __device__ __forceinline__ void find_tile(const WinArgs& a, int rows, int t, int
   }
 }
 
-// Is `row` one of a sequence's?
+// Is `row` one of a sequence's? The same row in all lanes, which look at 64 sequences at a time.
 __device__ __forceinline__ bool owned(const WinArgs& a, int row, int lane) {
   bool mine = false;
   for (int i = lane; i < a.n_seqs; i += 64) {
@@ -379,6 +379,27 @@ __device__ __forceinline__ bool owned(const WinArgs& a, int row, int lane) {
     mine = mine || (is_sequence(a, qs, ql, a.lens[i * 3 + 2]) && row >= qs && row < qs + ql);
   }
   return __ballot(mine) != 0;
+}
+
+// Zeroes the rows from `lo` on, up to 64 of them and below `hi`, that no sequence has, for one kv head's query heads: a lane looks
+// at one row, all sequences pass by.
+__device__ __forceinline__ void zero_rows(const WinArgs& a, int lo, int hi, int h, int lane) {
+  const int row = lo + lane;
+  bool mine = row >= hi;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    int qs = 0, ql = 0;
+    if (s0 + lane < a.n_seqs) {
+      qs = a.lens[(s0 + lane) * 3];
+      ql = a.lens[(s0 + lane) * 3 + 1];
+      if (!is_sequence(a, qs, ql, a.lens[(s0 + lane) * 3 + 2])) ql = 0;
+    }
+    const int n = a.n_seqs - s0 < 64 ? a.n_seqs - s0 : 64;
+    for (int j = 0; j < n; ++j) mine = mine || (unsigned)(row - __builtin_amdgcn_readlane(qs, j)) < (unsigned)__builtin_amdgcn_readlane(ql, j);
+  }
+  for (uint64_t rest = __ballot(!mine); rest != 0; rest &= rest - 1) {
+    const size_t head = (size_t)(lo + __builtin_ctzll(rest)) * a.n_q + (size_t)h * a.G;
+    for (int e = lane * 8; e < a.G * HD; e += 512) *reinterpret_cast<uint4*>(a.out + head * HD + e) = uint4{0, 0, 0, 0};
+  }
 }
 
 // A wave's state: QT tiles of 16 query rows, lane (fr, fq) has row fr of each.
@@ -611,11 +632,8 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
   int seq, tile, in_use;
   find_tile(a, ROWS, blockIdx.y, lane, seq, tile, in_use);
   if (a.zero_rest && a.splits == 1 && in_use < a.rows) {               // this block's share of the rows that may be nobody's
-    const int share = (a.rows + gridDim.y - 1) / gridDim.y;
-    for (int row = blockIdx.y * share + w; row < a.rows && row < (int)(blockIdx.y + 1) * share; row += 4)
-      if (!owned(a, row, lane))
-        for (int e = lane * 8; e < a.G * HD; e += 512)
-          *reinterpret_cast<uint4*>(a.out + ((size_t)row * a.n_q + (size_t)h * a.G) * HD + e) = uint4{0, 0, 0, 0};
+    const int share = (a.rows + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * share, hi = lo + share < a.rows ? lo + share : a.rows;
+    for (int row = lo + w * 64; row < hi; row += 256) zero_rows(a, row, hi, h, lane);
   }
   if (seq < 0) return;
   const int q_start = a.lens[seq * 3], q_len = a.lens[seq * 3 + 1], ctx = a.lens[seq * 3 + 2];
