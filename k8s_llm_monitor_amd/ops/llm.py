@@ -694,12 +694,22 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     return out
 
 
-def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int) -> Tuple[int, int]:
-    """(16-row tiles a wave, splits of the keys) of `paged_attn_prefill_window`, `reach` keys being the most that a query sees."""
-    if (rows * group // 192 + seqs) * n_kv >= 256:
+def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int, span: int) -> Tuple[int, int]:
+    """(16-row tiles a wave, splits of the keys) of `paged_attn_prefill_window`: `reach` keys are the most that a query sees, `span`
+    the most that a context has.
+
+    A block of 3 tiles a wave takes three times the rows for 2.1 times the time (1.7 and 0.8 us a 32-key step with the chip
+    full), one of a single tile leaves less idle where the last blocks run alone. MI355X, 32 query heads over 8 kv heads, one
+    whole prompt, whose first tiles see few keys: 2048 tokens (344 blocks of the large kind) 56 us with single tiles and 117
+    with three, 4096 (688) 183 and 234, 5000 (840) 268 and 287, 6144 (1032) 383 and 297. Chunks of a longer context, whose
+    tiles all see the same: 2048 queries behind 4000 keys (344) 156 and 181, the same with 64 heads (688) 293 and 264, 1200
+    with 64 heads (408) 180 and 138. Splits pay while single tiles leave CUs without a block: 16 queries over 4000 keys
+    11.8 us with 16 of them, 39 without; 500 queries 21.0 us without, 23.6 with 2."""
+    large = (rows * group // 192 + seqs) * n_kv
+    if large >= (380 if span > 1.5 * rows else 840):
         return 3, 1
     blocks = (-(-rows * group // 64) + seqs - 1) * n_kv
-    return 1, max(1, min(512 // blocks, (reach // 32 + 1) // 4, 32))
+    return 1, max(1, min(300 // blocks, (reach // 32 + 1) // 4, 16))
 
 
 def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -727,7 +737,7 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if zero_rest:
         out = q.new_empty((T, n_q * HEAD_DIM))
     window, sinks = min(window, _FAR), min(sinks, _FAR)
-    q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK))
+    q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK), width * BLOCK)
     part_o = part_ml = 0
     if splits > 1:
         scratch = torch.empty(T * n_q * splits * (HEAD_DIM + 2), dtype=torch.float32, device=q.device)
