@@ -8,6 +8,8 @@
 // gives 0. A masked key contributes nothing whatever its bytes are (stale slots, NaN, infinities).
 //
 // No reference counterpart (vLLM is a README bullet in the reference, README.md:73).
+#include <type_traits>
+
 #include "klm_launch.h"
 #include "llm_common.h"
 
@@ -33,7 +35,7 @@ struct WinArgs {
   float scale_log2;
 };
 
-// The keys a span of queries at positions [pos_a, pos_b] may see, as 32-key steps: the sinks' steps, then the window's.
+// The keys a span of queries at positions [pos_a, pos_b] may see, as steps of 32 keys: the sinks' steps, then the window's.
 struct Span {
   int lo, n_sink, lo_step, n;
   __device__ __forceinline__ int step(int i) const { return i < n_sink ? i : lo_step + (i - n_sink); }
@@ -65,49 +67,40 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t x) { return ((x & 0x7f80
 __device__ __forceinline__ uint32_t without_odd(uint32_t x) { return x & ~((odd_halves(x) >> 15) * 0xffffu); }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// One token per sequence. Block = (16 query heads of a kv head, sequence, split); its 4 waves take the 32-key steps of the
-// split in turn, K and V^T fragments straight from the cache into matrix operands (see llm_attention.hip for the operand
-// mapping), the next step's 16 KiB in flight.
+// One token per sequence: what bounds it is the cache that has to be read once. Block = (16 query heads of a kv head, sequence,
+// split); its 4 waves take the 32-key steps of the split in turn, loaded past the caches straight into matrix operands, the next
+// step's 16 KiB (e4m3: 8) in flight under this one's work. e4m3 stays raw until its turn: turned into bf16 as it came it would
+// be waited for at once. The operand mapping is llm_attention.hip's. Measured, 8 kv heads, window 4096: 128 sequences of up to
+// 8192 tokens 252 us, 5.4 TB/s (through the caches 257 us); 96 of e4m3, 118 us, 4.6 TB/s (64-key steps 121 us). The same loads
+// without products and softmax take 247 and 111 us.
 // ---------------------------------------------------------------------------------------------------------------------
-struct DFrags {
-  bf16x8 k[2][4];
-  bf16x8 v[8];
-  int p0, p1;            // the step's two pages, -1: none
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+template <bool KV8>
+struct Raw {
+  using V = std::conditional_t<KV8, u32x2, u32x4>;      // 8 tokens of a dim
+  u32x4 k[KV8 ? 4 : 8];  // bf16: tile i / 4 (tokens + 4), k-step i % 4; e4m3: tile i / 2, 64 dims i % 2
+  V v[8];
+  int pv;                // the page that this lane's V comes from, -1: none
 };
 
 template <bool KV8>
-__device__ __forceinline__ void load_step(const WinArgs& a, const int* table, int h, int step, int fr, int fq, DFrags& f) {
-  f.p0 = page_at(table, step * 2, a.width, a.pages);
-  f.p1 = page_at(table, step * 2 + 1, a.width, a.pages);
-  const size_t b0 = ((size_t)(f.p0 < 0 ? 0 : f.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(f.p1 < 0 ? 0 : f.p1) * a.n_kv + h) * BLK_ELEMS;
-  const size_t ko = ((fr >> 3) ? b1 : b0) + ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD;
-  const size_t vo = ((fq >> 1) ? b1 : b0) + fr * BLK + (fq & 1) * 8;
-  if (KV8) {
-    const uint8_t* kp = (const uint8_t*)a.kc + ko + fq * 16;
-    const uint8_t* vp = (const uint8_t*)a.vc + vo;
+__device__ __forceinline__ void load_raw(const WinArgs& a, int held, int j, int h, int fr, int fq, Raw<KV8>& f) {
+  constexpr int ES = KV8 ? 1 : 2;
+  const int pk = __shfl(held, j * 2 + (fr >> 3));
+  f.pv = __shfl(held, j * 2 + (fq >> 1));
+  const char* kp = (const char*)a.kc + ((size_t)(pk < 0 ? 0 : pk) * a.n_kv + h) * (BLK_ELEMS * ES);
+  const char* vp = (const char*)a.vc + ((size_t)(f.pv < 0 ? 0 : f.pv) * a.n_kv + h) * (BLK_ELEMS * ES);
+  kp += ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD * ES + fq * 16;
+  vp += (fr * BLK + (fq & 1) * 8) * ES;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(kp + t * 4 * HD + h2 * 64);
-        f.k[t][2 * h2] = fp8x8_to_bf16(raw.x, raw.y);
-        f.k[t][2 * h2 + 1] = fp8x8_to_bf16(raw.z, raw.w);
-      }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(vp + n * 16 * BLK);
-      f.v[n] = fp8x8_to_bf16(raw.x, raw.y);
-    }
-  } else {
-    const uint16_t* kp = (const uint16_t*)a.kc + ko + fq * 8;
-    const uint16_t* vp = (const uint16_t*)a.vc + vo;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) f.k[t][s] = *reinterpret_cast<const bf16x8*>(kp + t * 4 * HD + s * 32);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) f.v[n] = *reinterpret_cast<const bf16x8*>(vp + n * 16 * BLK);
+  for (int i = 0; i < (KV8 ? 4 : 8); ++i) {
+    const int off = KV8 ? (i >> 1) * 4 * HD + (i & 1) * 64 : ((i >> 2) * 4 * HD + (i & 3) * 32) * 2;
+    f.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + off));
   }
+#pragma unroll
+  for (int n = 0; n < 8; ++n) f.v[n] = __builtin_nontemporal_load(reinterpret_cast<const typename Raw<KV8>::V*>(vp + n * 16 * BLK * ES));
 }
 
 struct DAcc {
@@ -115,51 +108,51 @@ struct DAcc {
   float m, l;
 };
 
-// ctx: every row of the block stands at position ctx - 1, so all rows share one mask
-__device__ __forceinline__ void decode_step(DFrags& f, const bf16x8 (&qf)[4], int step, int fq, int ctx, int lo, int sinks,
-                                            float scale_log2, DAcc& a) {
+// ctx: every row of the block stands at position ctx - 1, so all rows share one mask.
+template <bool KV8>
+__device__ __forceinline__ void decode_step(Raw<KV8>& f, const bf16x8 (&qf)[4], int key, bool inside, int ctx, int lo, int sinks,
+                                             float scale_log2, DAcc& a) {
   f32x4 s0 = f32x4{0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[0][s], qf[s], s0, 0, 0, 0);
-    s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[1][s], qf[s], s1, 0, 0, 0);
+    bf16x8 k0, k1;
+    if constexpr (KV8) {
+      const u32x4 r0 = f.k[s >> 1], r1 = f.k[2 + (s >> 1)];
+      k0 = (s & 1) ? fp8x8_to_bf16(r0[2], r0[3]) : fp8x8_to_bf16(r0[0], r0[1]);
+      k1 = (s & 1) ? fp8x8_to_bf16(r1[2], r1[3]) : fp8x8_to_bf16(r1[0], r1[1]);
+    } else {
+      k0 = __builtin_bit_cast(bf16x8, f.k[s]);
+      k1 = __builtin_bit_cast(bf16x8, f.k[4 + s]);
+    }
+    s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[s], s0, 0, 0, 0);
+    s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[s], s1, 0, 0, 0);
   }
   float x[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    x[j] = s0[j];
-    x[j + 4] = s1[j];
+    x[j] = s0[j] * scale_log2;
+    x[j + 4] = s1[j] * scale_log2;
   }
-  const int k0 = step * 32;
-  const bool inside = k0 + 31 < ctx && (k0 >= lo || k0 + 31 < sinks) && f.p0 >= 0 && f.p1 >= 0;
+  uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
   if (!inside) {                                            // wave-uniform: the window's two ends and the last sink step
-    const int tk = k0 + fq * 8;
-    const bool page = ((fq >> 1) ? f.p1 : f.p0) >= 0;
-    uint32_t keep[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const bool see = page && tk + j < ctx && (tk + j >= lo || tk + j < sinks);
+      const bool see = f.pv >= 0 && key + j < ctx && (key + j >= lo || key + j < sinks);
       x[j] = see ? x[j] : -INFINITY;
-      keep[j >> 1] |= see ? (0xffffu << (16 * (j & 1))) : 0u;
-    }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {                           // a weight of 0 times a NaN would reach the sum: masked values go
-      uint4 u = __builtin_bit_cast(uint4, f.v[n]);
-      u = uint4{u.x & keep[0], u.y & keep[1], u.z & keep[2], u.w & keep[3]};
-      f.v[n] = __builtin_bit_cast(bf16x8, u);
+      if (!see) keep[j >> 1] &= (j & 1) ? 0xffffu : 0xffff0000u;
     }
   }
   float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
   mx = fmaxf(mx, __shfl_xor(mx, 16));
   mx = fmaxf(mx, __shfl_xor(mx, 32));
-  const float m_new = fmaxf(a.m, mx * scale_log2);
+  const float m_new = fmaxf(a.m, mx);
   const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
   const float alpha = fast_exp2(a.m - m_use);
   bf16x8 p;
   float rs = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float pj = fast_exp2(fmaf(x[j], scale_log2, -m_use));
+    const float pj = fast_exp2(x[j] - m_use);
     p[j] = (__bf16)pj;
     rs += pj;
   }
@@ -170,13 +163,20 @@ __device__ __forceinline__ void decode_step(DFrags& f, const bf16x8 (&qf)[4], in
     for (int n = 0; n < 8; ++n) a.o[n] *= alpha;
   }
 #pragma unroll
-  for (int n = 0; n < 8; ++n) a.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v[n], p, a.o[n], 0, 0, 0);
+  for (int n = 0; n < 8; ++n) {
+    u32x4 u;
+    if constexpr (KV8) u = __builtin_bit_cast(u32x4, fp8x8_to_bf16(f.v[n][0], f.v[n][1]));
+    else u = f.v[n];
+    if (!inside) u = u32x4{u[0] & keep[0], u[1] & keep[1], u[2] & keep[2], u[3] & keep[3]};      // a weight of 0 times a NaN would reach the sum
+    a.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u), p, a.o[n], 0, 0, 0);
+  }
 }
 
 constexpr int OPAD = HD + 4;
 
 template <bool KV8>
-__global__ __launch_bounds__(256) void window_decode_kernel(WinArgs a, int head_tiles) {
+__global__ __launch_bounds__(256, 2) void window_decode_kernel(WinArgs a, int head_tiles) {
+  constexpr int HELD = 32;
   __shared__ float sm_o[4][16][OPAD];
   __shared__ float sm_m[4][16], sm_l[4][16];
   const int h = blockIdx.x / head_tiles, ht = blockIdx.x % head_tiles, b = blockIdx.y, split = blockIdx.z;
@@ -188,31 +188,42 @@ __global__ __launch_bounds__(256) void window_decode_kernel(WinArgs a, int head_
   Span sp = make_span(ctx - 1, ctx - 1, a.window, a.sinks, a.width);
   if (ctx <= 0) sp.n = 0;
   const int sps = (sp.n + a.splits - 1) / a.splits;
-  const int i0 = split * sps, i1 = (i0 + sps) < sp.n ? (i0 + sps) : sp.n;
+  const int i0 = split * sps + w, i1 = (split + 1) * sps < sp.n ? (split + 1) * sps : sp.n;      // the wave's steps: i0, i0 + 4, ..
   const int row_head = ht * 16 + fr;
   const bool valid = row_head < a.G;
-  const uint16_t* qrow = a.q + (size_t)b * a.q_stride + ((size_t)h * a.G + (valid ? row_head : 0)) * HD;
-  bf16x8 qf[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    // fp8: a 16-byte K load carries 16 dims = two k-steps of the product, q follows that order
-    if (valid) qf[s] = *reinterpret_cast<const bf16x8*>(qrow + (KV8 ? (s >> 1) * 64 + fq * 16 + (s & 1) * 8 : s * 32 + fq * 8));
-    else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) qf[s][j] = (__bf16)0.f;
-  }
+  // a lane holds one page id of the wave's next HELD steps: the loads of a step wait for no table
+  int held = -1;
+  const auto hold = [&](int i) {
+    const int step = i + (lane >> 1) * 4;
+    held = step < i1 ? page_at(table, sp.step(step) * 2 + (lane & 1), a.width, a.pages) : -1;
+  };
   DAcc acc;
 #pragma unroll
   for (int n = 0; n < 8; ++n) acc.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   acc.m = -INFINITY;
   acc.l = 0.f;
-  if (i0 + w < i1) {
-    DFrags cur;
-    load_step<KV8>(a, table, h, sp.step(i0 + w), fr, fq, cur);
-    for (int i = i0 + w; i < i1; i += 4) {
-      DFrags nxt;
-      load_step<KV8>(a, table, h, sp.step(i + 4 < i1 ? i + 4 : i), fr, fq, nxt);
-      decode_step(cur, qf, sp.step(i), fq, ctx, sp.lo, a.sinks, a.scale_log2, acc);
+  if (i0 < i1) {
+    hold(i0);
+    Raw<KV8> cur, nxt;
+    load_raw<KV8>(a, held, 0, h, fr, fq, cur);
+    const uint16_t* qrow = a.q + (size_t)b * a.q_stride + ((size_t)h * a.G + (valid ? row_head : 0)) * HD;
+    bf16x8 qf[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      // e4m3: a 16-byte K load carries 16 dims = two k-steps of the product, q follows that order
+      u32x4 u = u32x4{0, 0, 0, 0};
+      if (valid) u = *reinterpret_cast<const u32x4*>(qrow + (KV8 ? (s >> 1) * 64 + fq * 16 + (s & 1) * 8 : s * 32 + fq * 8));
+      qf[s] = __builtin_bit_cast(bf16x8, u);
+    }
+    for (int i = i0, j = 0; i < i1; i += 4) {
+      if (++j == HELD) {
+        hold(i + 4);
+        j = 0;
+      }
+      if (i + 4 < i1) load_raw<KV8>(a, held, j, h, fr, fq, nxt);
+      const int k0 = sp.step(i) << 5, k1 = k0 + 31;
+      const bool inside = k1 < ctx && (k0 >= sp.lo || k1 < a.sinks) && __ballot(cur.pv < 0) == 0;
+      decode_step<KV8>(cur, qf, k0 + fq * 8, inside, ctx, sp.lo, a.sinks, a.scale_log2, acc);
       cur = nxt;
     }
   }
@@ -546,6 +557,48 @@ __device__ __forceinline__ void write_rows(const WinArgs& a, int64_t dst, int sp
       a.part_ml[at * 2] = m;
       a.part_ml[at * 2 + 1] = l;
     }
+  }
+}
+
+// A 32-key step's fragments straight from the cache, as decode takes them from a bf16 one.
+struct DFrags {
+  bf16x8 k[2][4];
+  bf16x8 v[8];
+  int p0, p1;            // the step's two pages, -1: none
+};
+
+template <bool KV8>
+__device__ __forceinline__ void load_step(const WinArgs& a, const int* table, int h, int step, int fr, int fq, DFrags& f) {
+  f.p0 = page_at(table, step * 2, a.width, a.pages);
+  f.p1 = page_at(table, step * 2 + 1, a.width, a.pages);
+  const size_t b0 = ((size_t)(f.p0 < 0 ? 0 : f.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(f.p1 < 0 ? 0 : f.p1) * a.n_kv + h) * BLK_ELEMS;
+  const size_t ko = ((fr >> 3) ? b1 : b0) + ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD;
+  const size_t vo = ((fq >> 1) ? b1 : b0) + fr * BLK + (fq & 1) * 8;
+  if (KV8) {
+    const uint8_t* kp = (const uint8_t*)a.kc + ko + fq * 16;
+    const uint8_t* vp = (const uint8_t*)a.vc + vo;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(kp + t * 4 * HD + h2 * 64);
+        f.k[t][2 * h2] = fp8x8_to_bf16(raw.x, raw.y);
+        f.k[t][2 * h2 + 1] = fp8x8_to_bf16(raw.z, raw.w);
+      }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(vp + n * 16 * BLK);
+      f.v[n] = fp8x8_to_bf16(raw.x, raw.y);
+    }
+  } else {
+    const uint16_t* kp = (const uint16_t*)a.kc + ko + fq * 8;
+    const uint16_t* vp = (const uint16_t*)a.vc + vo;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) f.k[t][s] = *reinterpret_cast<const bf16x8*>(kp + t * 4 * HD + s * 32);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) f.v[n] = *reinterpret_cast<const bf16x8*>(vp + n * 16 * BLK);
   }
 }
 

@@ -645,6 +645,13 @@ def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q
         _i32(block_tables, lens)
 
 
+def pick_window_splits(blocks: int, reach: int) -> int:
+    """Splits of `paged_attn_decode_window` for `blocks` (sequence, 16 heads of a kv head) pairs that see up to `reach` keys each:
+    two blocks a CU; about 2048 keys a block at most, for even ends where blocks queue (1024 of 4096 keys: 1 split 261 us, 2 252;
+    512 of 1024 keys: 1 split 47 us, 2 50); 64 keys at least; 24 splits at most (each writes a part that the join reads)."""
+    return max(1, min(max(-(-512 // max(1, blocks)), (reach + 1024) // 2048), reach // 64, 24))
+
+
 def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                              ctx_lens: torch.Tensor, scale: float, n_q: int, window: int, sinks: int = 0,
                              out: Optional[torch.Tensor] = None, num_splits: int = 0,
@@ -674,7 +681,7 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     if B == 0:
         return out
     window, sinks = min(window, _FAR), min(sinks, _FAR)
-    splits = num_splits or pick_splits(B, n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
+    splits = num_splits or pick_window_splits(B * n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
     part_o = part_ml = 0
     if splits > 1:
         if workspace is None:
