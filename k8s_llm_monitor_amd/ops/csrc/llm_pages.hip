@@ -26,8 +26,9 @@ struct PageArgs {
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
-// One 16-byte load and store a thread, both past the caches: a page is not read again soon by whoever copies it. MI355X, 683 pages
-// of 32 layers of 32 KiB, read and written: see the figures at the launcher.
+// One 16-byte load and store a thread, both past the caches: a page is not read again soon by whoever copies it. MI355X, read and
+// written: 683 pages of 32 layers, 32 KiB each in K and in V, 539 us, 5.3 TB/s (through the caches, with 64 bytes a thread in
+// one pass, 571 us); 250 e4m3 pages of 80 layers 209 us, 6.3 TB/s (241 us). A torch copy of one large tensor reaches 6.6 TB/s.
 __global__ __launch_bounds__(256) void copy_pages_kernel(PageArgs a, PagePairs p) {
   const int src = p.src[blockIdx.y], dst = p.dst[blockIdx.y], layer = blockIdx.z >> 1;
   const bool v = blockIdx.z & 1;

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from array import array
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -765,12 +766,13 @@ _PAGES_ARGS = struct.Struct("6P6i")             # klm_pages_args
 
 def _page_shape(k: torch.Tensor, v: torch.Tensor) -> Tuple[int, int, int]:
     """(layers, blocks, n_kv) of a cache [layers, blocks, n_kv, 16, 128] / [.., 128, 16], or of one layer of it."""
-    if k.dim() == 4 and v.dim() == 4:
-        k, v = k[None], v[None]
-    if k.dim() != 5 or tuple(k.shape[3:]) != (BLOCK, HEAD_DIM) or tuple(v.shape) != (*k.shape[:3], HEAD_DIM, BLOCK) or k.dtype != v.dtype or \
-            not k.is_contiguous() or not v.is_contiguous() or min(k.shape) < 1:
+    ks, vs = tuple(k.shape), tuple(v.shape)
+    if len(ks) == 4:
+        ks, vs = (1, *ks), (1, *vs)
+    if len(ks) != 5 or ks[3:] != (BLOCK, HEAD_DIM) or vs != (*ks[:3], HEAD_DIM, BLOCK) or k.dtype != v.dtype or \
+            not k.is_contiguous() or not v.is_contiguous() or 0 in ks:
         raise KlmOpsError(f"copy_pages: cache shapes K {tuple(k.shape)} {k.dtype} V {tuple(v.shape)} {v.dtype}")
-    return int(k.shape[0]), int(k.shape[1]), int(k.shape[2])
+    return ks[:3]
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -806,16 +808,31 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs: Sequence[Tup
         raise KlmOpsError("copy_pages: tensors on different devices")
     if k_cache.is_cuda:
         _kv8(k_cache)
-    p = _page_pairs(pairs, src_nb, nb, same)
+    p = _few_pairs(pairs, src_nb, nb, same) if type(pairs) is list and len(pairs) <= 32 else None
+    if p is None:
+        p = _page_pairs(pairs, src_nb, nb, same)
     if not len(p):
         return
     if not k_cache.is_cuda:
         ref.copy_pages(k_cache, v_cache, p, k_src, v_src)
         return
-    rc = _call(_lib().klm_copy_pages, _PAGES_ARGS.pack(k_src.data_ptr(), v_src.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), p.ctypes.data,
-                                                       _stream(k_cache), len(p), L, src_nb, nb, n_kv, k_cache.element_size()), k_cache)
+    rc = _call(_lib().klm_copy_pages, _PAGES_ARGS.pack(k_src.data_ptr(), v_src.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                       p.__array_interface__["data"][0], _stream(k_cache), len(p), L, src_nb, nb, n_kv, k_cache.element_size()), k_cache)
     if rc:
         _check(rc, f"klm_copy_pages(pairs={len(p)},layers={L})")
+
+
+def _few_pairs(pairs: list, src_nb: int, nb: int, same: bool) -> Optional[np.ndarray]:
+    """`_page_pairs` of a short list, without the cost of numpy's calls (4 pairs: the whole call 9.0 us instead of 14.9; 64 pairs
+    take both as long). None: something is out of order, `_page_pairs` sorts it out or says what it is."""
+    try:
+        to = {d: s for s, d in pairs}
+        if len(to) != len(pairs) or (same and not to.keys().isdisjoint(to.values())) or \
+                not all(-1 <= s < src_nb and 0 <= d < nb for d, s in to.items()):
+            return None
+        return np.frombuffer(array("i", [x for pair in pairs for x in pair]), dtype=np.int32).reshape(-1, 2)
+    except (TypeError, ValueError, OverflowError):
+        return None
 
 
 def _page_pairs(pairs, src_nb: int, nb: int, same: bool) -> np.ndarray:
