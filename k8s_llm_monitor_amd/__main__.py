@@ -104,6 +104,7 @@ def _cmd_serve_llm_replicas(a) -> int:
              "--kv-blocks", str(a.kv_blocks), "--kv-fraction", str(a.kv_fraction), "--decode-weights", a.decode_weights,
              "--kv-cache-dtype", a.kv_cache_dtype, "--load-rps", str(a.load_rps / a.gpus), "--prompt-len", str(a.prompt_len),
              "--output-len", str(a.output_len), "--max-num-batched-tokens", str(a.max_num_batched_tokens)] + \
+        (["--window", str(a.window), "--sinks", str(a.sinks)] if a.window or a.sinks else []) + \
         (["--no-graphs"] if a.no_graphs else []) + (["--no-mixed-batches"] if a.no_mixed_batches else [])
     kind = "cpu" if a.device == "cpu" else "cuda"
     base = a.replica_base_port or a.port + 1
@@ -230,7 +231,8 @@ def _cmd_serve_llm(a) -> int:
     eng = Engine(EngineConfig(model=a.model, device=device, max_num_seqs=a.max_num_seqs, max_model_len=a.max_model_len,
                               kv_blocks=a.kv_blocks, kv_fraction=a.kv_fraction, use_graphs=not a.no_graphs,
                               decode_weights=a.decode_weights, kv_cache_dtype=a.kv_cache_dtype,
-                              max_num_batched_tokens=a.max_num_batched_tokens, mixed_batches=not a.no_mixed_batches), tp=tp)
+                              max_num_batched_tokens=a.max_num_batched_tokens, mixed_batches=not a.no_mixed_batches,
+                              window=a.window, sinks=a.sinks), tp=tp)
     eng.warmup()
     if tp is not None and tp.rank != 0:
         for sig in (signal.SIGINT, signal.SIGTERM):
@@ -329,6 +331,9 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
                    help="fp8: W8A16 weight copies for decode up to batch 128 (half the bytes per token; costs half the model size in HBM)")
     p.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "fp8"],
                    help="fp8: e4m3 KV cache, twice the tokens per GB and half the attention bytes")
+    p.add_argument("--window", type=int, default=0,
+                   help="attend to the last N tokens only; the cache blocks behind them are given back (0: as the model says)")
+    p.add_argument("--sinks", type=int, default=0, help="with --window: and to the first N tokens")
     p.add_argument("--load-rps", type=float, default=0.0, help="built-in open-loop load (requests per second)")
     p.add_argument("--prompt-len", type=int, default=512)
     p.add_argument("--output-len", type=int, default=128)

@@ -53,6 +53,8 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     eps: float = 1e-5
     max_pos: int = 8192
+    window: int = 0        # a token attends to the last `window` tokens, its own among them (0: to all) ...
+    sinks: int = 0         # ... and to the first `sinks` of its context
 
     @property
     def q_dim(self) -> int:
@@ -81,6 +83,8 @@ class LlamaConfig:
 
     def flops_per_token(self, ctx: int = 0) -> float:
         """Forward FLOPs of one token (GEMMs + attention over `ctx` keys), embedding lookup excluded."""
+        if self.window:
+            ctx = min(ctx, self.window + self.sinks)
         gemm = 2.0 * (self.params() - self.vocab * self.hidden)
         attn = 4.0 * self.layers * self.n_q * HEAD_DIM * ctx
         return gemm + attn
@@ -135,7 +139,7 @@ class DecodeMeta:
 class PrefillMeta:
     block_tables: torch.Tensor          # int32 [S, max_blocks]
     seq_info: torch.Tensor              # int32 [S, 3] = (q_start, q_len, ctx_len)
-    tiles: torch.Tensor                 # int32 [n_tiles, 2], built for `q_tiles`
+    tiles: torch.Tensor                 # int32 [n_tiles, 2], built for `q_tiles` (not looked at by a model with a window)
     last_rows: torch.Tensor             # int64 [S]: row of each sequence's last token
     q_tiles: int = llm.PREFILL_Q_TILES
 
@@ -449,14 +453,32 @@ class LlamaModel:
         ok = batch <= self.skinny_rows() and c.hidden % 128 == 0 and c.ffn % 128 == 0 and c.vocab % 16 == 0
         return ok and (not self.fp8_decode or (c.hidden % 64 == 0 and c.ffn % 64 == 0))
 
-    def decode(self, tokens, positions, slots, cache: KVCache, meta: DecodeMeta, logits: bool = False) -> torch.Tensor:
+    def _attend_token(self, qkv, kc, vc, meta: DecodeMeta, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of one token per sequence, with the model's window if it has one."""
+        cfg = self.lcfg
+        if cfg.window:
+            return llm.paged_attn_decode_window(qkv, kc, vc, meta.block_tables, meta.ctx_lens, self.scale, cfg.n_q, cfg.window, cfg.sinks,
+                                                out=out, workspace=meta.workspace)
+        return llm.paged_attn_decode(qkv, kc, vc, meta.block_tables, meta.ctx_lens, self.scale, cfg.n_q, out=out,
+                                     num_splits=meta.num_splits, workspace=meta.workspace)
+
+    def _attend_prompts(self, qkv, kc, vc, meta: PrefillMeta, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        cfg = self.lcfg
+        if cfg.window:
+            return llm.paged_attn_prefill_window(qkv, kc, vc, meta.block_tables, meta.seq_info, self.scale, cfg.n_q, cfg.window, cfg.sinks,
+                                                 out=out)
+        return llm.paged_attn_prefill(qkv, kc, vc, meta.block_tables, meta.seq_info, meta.tiles, self.scale, cfg.n_q, out=out,
+                                      q_tiles=meta.q_tiles)
+
+    def decode(self, tokens, positions, slots, cache: KVCache, meta: DecodeMeta, logits: bool = False,
+               rules: Optional[llm.LogitRules] = None) -> torch.Tensor:
         """One token per sequence -> greedy next token ids [B] (int64), or the logits [B, vocab].
-        `positions` are `meta.ctx_lens - 1` (the token being decoded is the last of its context). Capture-safe."""
+        `positions` are `meta.ctx_lens - 1` (the token being decoded is the last of its context). `rules`: the choice follows
+        them (ids and masks in the whole vocabulary's numbers, whatever part of it this rank holds). Capture-safe."""
         cfg = self.lcfg
 
         def attend(qkv, kc, vc):
-            return llm.paged_attn_decode(qkv, kc, vc, meta.block_tables, meta.ctx_lens, self.scale, cfg.n_q,
-                                         num_splits=meta.num_splits, workspace=meta.workspace)
+            return self._attend_token(qkv, kc, vc, meta)
 
         def attend_rope(qkv, kc, vc):
             # launch-bound regime: rotation and cache write ride inside the attention kernel (one launch less per layer)
@@ -464,7 +486,7 @@ class LlamaModel:
                                               cfg.n_q, num_splits=meta.num_splits, workspace=meta.workspace)
 
         if self.skinny(tokens.shape[0]):
-            fused = self.fused_rope and self.device.type == "cuda" and cache.k.dtype == torch.bfloat16
+            fused = self.fused_rope and self.device.type == "cuda" and cache.k.dtype == torch.bfloat16 and not cfg.window
             h = self._stack_skinny(tokens, positions, slots, cache, attend_rope if fused else attend, rope=not fused)
             if self.fp8_decode:
                 out = llm.skinny_linear(h, self.lm_head8, rms=True, eps=cfg.eps, weight_scale=self.lm_head_s, tiled=True)
@@ -472,48 +494,53 @@ class LlamaModel:
                 out = llm.skinny_linear(h, self.lm_head, rms=True, eps=cfg.eps)
         else:
             out = torch.matmul(self._trunk(tokens, positions, slots, cache, attend), self.lm_head.t())
-        return self._sample(out, logits)
+        return self._sample(out, logits, rules)
 
-    def _sample(self, out: torch.Tensor, logits: bool) -> torch.Tensor:
-        """Local logits [B, vocab / world] -> greedy token ids [B] (or the full logits [B, vocab])."""
+    def _sample(self, out: torch.Tensor, logits: bool, rules: Optional[llm.LogitRules] = None) -> torch.Tensor:
+        """Local logits [B, vocab / world] -> greedy token ids [B] (or the full logits [B, vocab], which no rules touch)."""
         tp = self.tp
         if tp.world == 1:
+            if rules is not None and not logits:
+                return llm.choose_tokens(out, rules)[0]
             return out if logits else out.argmax(dim=-1)
         B, vl = out.shape
         if logits:
             return tp.all_gather(out.contiguous()).permute(1, 0, 2).reshape(B, tp.world * vl)
         # every rank offers its best (value, global id); ids fit fp32 exactly (< 2^24); rows padded to 16 bytes
-        vals, idx = out.float().max(dim=-1)
+        if rules is None:
+            vals, idx = out.float().max(dim=-1)
+            idx = idx + tp.rank * vl
+        else:
+            # -1: the rules allow no token of this rank's part; any token that another rank may choose goes before that
+            idx, vals = llm.choose_tokens(out, rules, first_token=tp.rank * vl)
+            vals = torch.where(idx >= 0, vals.clamp(min=torch.finfo(torch.float32).min), -torch.inf)
         cand = torch.zeros((B + (B & 1), 2), dtype=torch.float32, device=out.device)
         cand[:B, 0] = vals
-        cand[:B, 1] = (idx + tp.rank * vl).float()
+        cand[:B, 1] = idx.float()
         allc = tp.all_gather(cand)                                   # [world, B', 2]: the same bits on every rank
         best = allc[:, :B, 0].argmax(dim=0)
         return allc[:, :B, 1].gather(0, best[None])[0].long()
 
     def prefill(self, tokens, positions, slots, cache: KVCache, meta: PrefillMeta, logits: bool = False,
-                riders: Optional[DecodeMeta] = None) -> torch.Tensor:
+                riders: Optional[DecodeMeta] = None, rules: Optional[llm.LogitRules] = None) -> torch.Tensor:
         """Variable-length batch of prompts (or prompt chunks) -> next token id of each row in `meta.last_rows`
         (or the logits of those rows). `riders`: the last ``riders.block_tables.shape[0]`` rows are one decode token each
         of running sequences (a mixed batch): they share the projections with the chunks and attend through the
-        decode kernel."""
+        decode kernel. `rules`: of the rows in `meta.last_rows`, as in `decode`."""
         cfg = self.lcfg
         n_ride = 0 if riders is None else riders.block_tables.shape[0]
         n_chunk = tokens.shape[0] - n_ride
 
         def attend(qkv, kc, vc):
             if not n_ride:
-                return llm.paged_attn_prefill(qkv, kc, vc, meta.block_tables, meta.seq_info, meta.tiles, self.scale,
-                                              cfg.n_q, q_tiles=meta.q_tiles)
+                return self._attend_prompts(qkv, kc, vc, meta)
             o = torch.empty((qkv.shape[0], cfg.q_dim), dtype=qkv.dtype, device=qkv.device)
-            llm.paged_attn_prefill(qkv[:n_chunk], kc, vc, meta.block_tables, meta.seq_info, meta.tiles, self.scale,
-                                   cfg.n_q, out=o[:n_chunk], q_tiles=meta.q_tiles)
-            llm.paged_attn_decode(qkv[n_chunk:], kc, vc, riders.block_tables, riders.ctx_lens, self.scale, cfg.n_q,
-                                  out=o[n_chunk:], num_splits=riders.num_splits, workspace=riders.workspace)
+            self._attend_prompts(qkv[:n_chunk], kc, vc, meta, out=o[:n_chunk])
+            self._attend_token(qkv[n_chunk:], kc, vc, riders, out=o[n_chunk:])
             return o
 
         x = self._trunk(tokens, positions, slots, cache, attend)
-        return self._sample(self._head(x[meta.last_rows]), logits)
+        return self._sample(self._head(x[meta.last_rows]), logits, rules)
 
     def _head(self, x: torch.Tensor) -> torch.Tensor:
         """The lm_head on already-normed rows (prefill: the prompts' last rows). Up to 16 rows: one pass of the skinny

@@ -443,6 +443,15 @@ struct Scores {
   f32x4 s[QT][2];
 };
 
+// Weights 2 c and 2 c + 1 of tile t's exponents. The sum is taken of the rounded weights, two at a time: they are what meets V.
+template <int QT>
+__device__ __forceinline__ void weights(Rows<QT>& r, const float (&x)[QT][8], int t, int c, bf16x8& p) {
+  const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][2 * c]), (__bf16)fast_exp2(x[t][2 * c + 1])};
+  p[2 * c] = two[0];
+  p[2 * c + 1] = two[1];
+  r.l[t] = __builtin_amdgcn_fdot2_f32_bf16(two, bf16x2{(__bf16)1.f, (__bf16)1.f}, r.l[t], false);
+}
+
 template <int QT>
 __device__ __forceinline__ void part_a(const char* st, int lane, Rows<QT>& r, const float (&x)[QT][8], Scores<QT>& s, bf16x8 (&p)[QT]) {
   const int fr = lane & 15, fq = lane >> 4;
@@ -457,11 +466,7 @@ __device__ __forceinline__ void part_a(const char* st, int lane, Rows<QT>& r, co
     for (int t = 0; t < QT; ++t) {
       s.s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s.s[t][0], 0, 0, 0);
       s.s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s.s[t][1], 0, 0, 0);
-      // the sum is taken of the rounded weights, two at a time: they are what meets V
-      const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][2 * c]), (__bf16)fast_exp2(x[t][2 * c + 1])};
-      p[t][2 * c] = two[0];
-      p[t][2 * c + 1] = two[1];
-      r.l[t] = __builtin_amdgcn_fdot2_f32_bf16(two, bf16x2{(__bf16)1.f, (__bf16)1.f}, r.l[t], false);
+      weights<QT>(r, x, t, c, p[t]);
     }
   }
 }
@@ -509,6 +514,7 @@ __device__ __forceinline__ void move_maximum(Rows<QT>& r, float (&x)[QT][8], flo
   if (__ballot(moves) == 0) return;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
+    if (__ballot(mx[t] > r.lim[t]) == 0) continue;                     // a tile's numbers do not hang on the wave's others
     mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 16));
     mx[t] = fmaxf(mx[t], __shfl_xor(mx[t], 32));
     const bool first = r.lim[t] < 0.f, seen = mx[t] > -INFINITY;
@@ -560,118 +566,81 @@ __device__ __forceinline__ void write_rows(const WinArgs& a, int64_t dst, int sp
   }
 }
 
-// A 32-key step's fragments straight from the cache, as decode takes them from a bf16 one.
-struct DFrags {
-  bf16x8 k[2][4];
-  bf16x8 v[8];
-  int p0, p1;            // the step's two pages, -1: none
-};
-
+// 8 values of the cache as bf16
 template <bool KV8>
-__device__ __forceinline__ void load_step(const WinArgs& a, const int* table, int h, int step, int fr, int fq, DFrags& f) {
-  f.p0 = page_at(table, step * 2, a.width, a.pages);
-  f.p1 = page_at(table, step * 2 + 1, a.width, a.pages);
-  const size_t b0 = ((size_t)(f.p0 < 0 ? 0 : f.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(f.p1 < 0 ? 0 : f.p1) * a.n_kv + h) * BLK_ELEMS;
-  const size_t ko = ((fr >> 3) ? b1 : b0) + ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD;
-  const size_t vo = ((fq >> 1) ? b1 : b0) + fr * BLK + (fq & 1) * 8;
+__device__ __forceinline__ bf16x8 load8(const void* cache, size_t at) {
   if (KV8) {
-    const uint8_t* kp = (const uint8_t*)a.kc + ko + fq * 16;
-    const uint8_t* vp = (const uint8_t*)a.vc + vo;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(kp + t * 4 * HD + h2 * 64);
-        f.k[t][2 * h2] = fp8x8_to_bf16(raw.x, raw.y);
-        f.k[t][2 * h2 + 1] = fp8x8_to_bf16(raw.z, raw.w);
-      }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(vp + n * 16 * BLK);
-      f.v[n] = fp8x8_to_bf16(raw.x, raw.y);
-    }
-  } else {
-    const uint16_t* kp = (const uint16_t*)a.kc + ko + fq * 8;
-    const uint16_t* vp = (const uint16_t*)a.vc + vo;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < 4; ++s) f.k[t][s] = *reinterpret_cast<const bf16x8*>(kp + t * 4 * HD + s * 32);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) f.v[n] = *reinterpret_cast<const bf16x8*>(vp + n * 16 * BLK);
+    const uint2 raw = *reinterpret_cast<const uint2*>((const uint8_t*)cache + at);
+    return fp8x8_to_bf16(raw.x, raw.y);
   }
+  return *reinterpret_cast<const bf16x8*>((const uint16_t*)cache + at);
 }
 
-// One 16-row tile again, from the cache and by itself, where V holds NaN or infinities that some rows see and others do not:
-// they leave the matrix product, and the rows that see them get them back. Rare and slow: a wave's steps one after another.
-template <bool KV8>
+// One 16-row tile again, from the cache and by themselves, where V holds NaN or infinities that some rows see and others do not:
+// they leave the matrix product, and the rows that see them get them back. Rare and slow: one step after another, every load
+// waited for. Each number is made as the fast loop makes it, so what a masked place holds does not move a single bit.
+template <bool KV8, typename Inside>
 __device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table, int h, const Span& sp, int i0, int i1, int split, int lane,
-                                             const uint16_t* qrow, int pos, int64_t dst) {
+                                             const uint16_t* qrow, int pos, int64_t dst, const Inside& is_inside) {
   const int fr = lane & 15, fq = lane >> 4;
-  bf16x8 q[4];
+  Rows<1> r;
+  r.pos[0] = pos;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int c = 0; c < 4; ++c) {
     uint4 u = uint4{0, 0, 0, 0};
-    if (dst >= 0) u = *reinterpret_cast<const uint4*>(qrow + (KV8 ? (s >> 1) * 64 + fq * 16 + (s & 1) * 8 : s * 32 + fq * 8));
-    q[s] = __builtin_bit_cast(bf16x8, u);
+    if (dst >= 0) u = *reinterpret_cast<const uint4*>(qrow + c * 32 + fq * 8);
+    r.q[0][c] = __builtin_bit_cast(bf16x8, u);
   }
-  f32x4 o[8];
 #pragma unroll
-  for (int n = 0; n < 8; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int n = 0; n < 8; ++n) r.o[0][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  r.lim[0] = -INFINITY;
+  r.shift[0] = 0.f;
+  r.l[0] = 0.f;
 #pragma unroll 1
   for (int i = i0; i < i1; ++i) {
     const int step = sp.step(i), key = step * 32 + fq * 8;
-    DFrags f;
-    load_step<KV8>(a, table, h, step, fr, fq, f);
+    const Pages2 pg{page_at(table, step * 2, a.width, a.pages), page_at(table, step * 2 + 1, a.width, a.pages)};
+    const size_t b0 = ((size_t)(pg.p0 < 0 ? 0 : pg.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(pg.p1 < 0 ? 0 : pg.p1) * a.n_kv + h) * BLK_ELEMS;
+    const size_t ko = ((fr >> 3) ? b1 : b0) + ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD + fq * 8;
+    const size_t vo = ((fq >> 1) ? b1 : b0) + fr * BLK + (fq & 1) * 8;
     f32x4 s0 = f32x4{0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[0][s], q[s], s0, 0, 0, 0);
-      s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.k[1][s], q[s], s1, 0, 0, 0);
+    for (int c = 0; c < 4; ++c) {
+      s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(load8<KV8>(a.kc, ko + c * 32), r.q[0][c], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(load8<KV8>(a.kc, ko + 4 * HD + c * 32), r.q[0][c], s1, 0, 0, 0);
     }
-    const int up = ((fq >> 1) ? f.p1 : f.p0) >= 0 ? pos - key : -1, down = pos - key - a.window, sink = a.sinks - key;
-    float x[8], mx = -INFINITY;
+    float x[1][8], mx[1];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[0][j] = fmaf(j < 4 ? s0[j & 3] : s1[j & 3], a.scale_log2, r.shift[0]);
+    mx[0] = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[0][4], x[0][5]), fmaxf(x[0][6], x[0][7])));
+    if (!is_inside(step, pg)) mask_step<1>(a, step, pg, lane, r, x, mx);
+    move_maximum<1>(r, x, mx);
+    const int up = ((fq >> 1) ? pg.p1 : pg.p0) >= 0 ? pos - key : -1, down = pos - key - a.window, sink = a.sinks - key;
+    bf16x8 p;
     uint32_t ones[4] = {0u, 0u, 0u, 0u};                               // 1 for a key that the row sees, as bf16 pairs
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool see = j <= up && (j > down || j < sink);
-      x[j] = see ? (j < 4 ? s0[j & 3] : s1[j & 3]) : -INFINITY;
-      ones[j >> 1] |= see ? 0x3f80u << (16 * (j & 1)) : 0u;
-      mx = fmaxf(mx, x[j]);
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float m_new = fmaxf(m, mx * a.scale_log2), shift = m_new == -INFINITY ? 0.f : -m_new;
-    const float alpha = fast_exp2(m + shift);
-    m = m_new;
-    l *= alpha;
-    bf16x8 p;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float pj = fast_exp2(fmaf(x[j], a.scale_log2, shift));
-      p[j] = (__bf16)pj;
-      l += pj;
-    }
+    for (int j = 0; j < 8; ++j) ones[j >> 1] |= j <= up && (j > down || j < sink) ? 0x3f80u << (16 * (j & 1)) : 0u;
     const bf16x8 one = __builtin_bit_cast(bf16x8, uint4{ones[0], ones[1], ones[2], ones[3]});
 #pragma unroll
+    for (int c = 0; c < 4; ++c) weights<1>(r, x, 0, c, p);
+#pragma unroll
     for (int n = 0; n < 8; ++n) {
-      uint4 u = __builtin_bit_cast(uint4, f.v[n]);
-      const uint4 marks = uint4{odd_marks(u.x), odd_marks(u.y), odd_marks(u.z), odd_marks(u.w)};
+      const uint4 u = __builtin_bit_cast(uint4, load8<KV8>(a.vc, vo + n * 16 * BLK));
+      const bf16x8 marks = __builtin_bit_cast(bf16x8, uint4{odd_marks(u.x), odd_marks(u.y), odd_marks(u.z), odd_marks(u.w)});
+      const bf16x8 v = __builtin_bit_cast(bf16x8, uint4{without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w)});
       // how many of them each row sees in each dim: exact in fp32
-      const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, marks), one, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-      u = uint4{without_odd(u.x), without_odd(u.y), without_odd(u.z), without_odd(u.w)};
-      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u), p, o[n] * alpha, 0, 0, 0);
+      const f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks, one, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      r.o[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p, r.o[0][n], 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int all = (int)c[j], neg = (all >> 6) & 63, inf = all & 63;
-        o[n][j] += all >= 4096 || (neg && inf) ? NAN : neg ? -INFINITY : inf ? INFINITY : 0.f;
+        if (all) r.o[0][n][j] += all >= 4096 || (neg && inf) ? NAN : neg ? -INFINITY : INFINITY;
       }
     }
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  write_rows(a, dst, split, fq, o, m, l);
+  r.l[0] += __shfl_xor(r.l[0], 16);
+  r.l[0] += __shfl_xor(r.l[0], 32);
+  write_rows(a, dst, split, fq, r.o[0], r.lim[0] > 0.f ? -r.shift[0] : -INFINITY, r.l[0]);
 }
 
 template <int QT, bool KV8>
@@ -730,6 +699,11 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     r.l[t] = 0.f;
   }
 
+  // does every row of the wave see all of a step? (Rows that are none see what they like then: they are not written.)
+  const auto is_inside = [&](int step, Pages2 pg) {
+    const int k0 = step * 32;
+    return k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && pg.p0 >= 0 && pg.p1 >= 0;
+  };
   bool odd = false;
   if (i0 < i1) {
     const int last = i1 - 1;
@@ -737,10 +711,6 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     const unsigned ko = (tok & 15) * 256 + (((lane & 15) ^ k_key(tok)) << 4);
     const unsigned vo = ((w & 1) * 64 + (lane >> 5) * 16 + (lane & 15)) * 32 + ((lane >> 4) & 1) * 16;
     const auto step_of = [&](int i) { return sp.step(i < last ? i : last); };      // past the last step: that one again, unused
-    const auto is_inside = [&](int step, Pages2 pg) {
-      const int k0 = step * 32;
-      return k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && pg.p0 >= 0 && pg.p1 >= 0;
-    };
     // Pages of step i + 1, i + 2 and i + 3. At step i its V and the K of i + 1 are in LDS, i + 2 is on its way, and i + 3 takes the
     // place of i - 1, which all waves have left at the barrier.
     // The table's entries for 32 steps at a time lie in one register, a lane each: looking them up in the loop through the scalar
@@ -802,7 +772,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[t][j] = (j < 4 ? s.s[t][0][j & 3] : s.s[t][1][j & 3]) * a.scale_log2;
+          x[t][j] = fmaf(j < 4 ? s.s[t][0][j & 3] : s.s[t][1][j & 3], a.scale_log2, r.shift[t]);
           mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
         }
     }
@@ -850,7 +820,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
       const bool valid = token < q_len;
       const size_t row = q_start + (valid ? token : 0), head = (size_t)h * G + g;
       careful_tile<KV8>(a, table, h, sp, i0, i1, split, lane, a.q + row * a.q_stride + head * HD, valid ? first + token : -1,
-                        valid ? (int64_t)(row * a.n_q + head) : -1);
+                        valid ? (int64_t)(row * a.n_q + head) : -1, is_inside);
     }
     return;
   }

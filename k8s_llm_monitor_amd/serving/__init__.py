@@ -7,3 +7,4 @@ this package.
 """
 from .engine import BlockAllocator, Engine, EngineConfig, Request  # noqa: F401
 from .metrics import EngineMetrics, Histogram, exact_quantile  # noqa: F401
+from .rules import RuleStore, TokenRules  # noqa: F401

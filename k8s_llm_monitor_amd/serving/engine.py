@@ -20,13 +20,17 @@ Scheduling (one `step()` = one model launch):
      re-enters the queue at the front and is recomputed from prompt + generated tokens.
 Decode runs from a hipGraph captured per batch-size bucket (launch-bound otherwise: ~10 kernel
 launches per layer); the graph's inputs are static device buffers that each step refills.
+
+A model with a window (`LlamaConfig.window`, or `EngineConfig.window`) never looks at pages behind it again: a sequence gives
+them back as it goes on, those of its sinks excepted. A request may carry rules on its tokens (serving/rules.py): launches with
+such a request choose with `ops.llm.choose_tokens`, all others as without.
 """
 from __future__ import annotations
 
 import threading
 import time
 from collections import deque
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Callable, Deque, Dict, List, Optional, Sequence
 
 import numpy as np
@@ -35,6 +39,7 @@ import torch
 from ..models.llama import BLOCK, PRESETS, DecodeMeta, KVCache, LlamaConfig, LlamaModel, PrefillMeta
 from ..ops import llm
 from .metrics import EngineMetrics
+from .rules import RuleStore, TokenRules
 
 
 @dataclass
@@ -50,6 +55,8 @@ class EngineConfig:
     kv_cache_dtype: str = "bf16"       # "fp8": e4m3 KV cache (half the bytes per token; prefill then uses the register kernel)
     decode_weights: str = "bf16"       # "fp8": W8A16 copies for decode up to batch 128 (LlamaModel.enable_fp8_decode)
     mixed_batches: bool = True         # running sequences decode inside prefill launches instead of waiting for them
+    window: int = 0                    # attention to the last `window` tokens and the first `sinks` (0: as the model says)
+    sinks: int = 0
     seed: int = 0
 
 
@@ -74,7 +81,8 @@ class BlockAllocator:
         return out
 
     def release(self, blocks: Sequence[int]) -> None:
-        self._free.extend(blocks)
+        """-1 (a block given back before) is passed over."""
+        self._free.extend(b for b in blocks if b >= 0)
 
 
 @dataclass
@@ -91,6 +99,9 @@ class Request:
     preempted: int = 0
     prefilled: int = 0                # tokens of prompt + out whose K/V are in the cache (chunked prefill)
     error: Optional[str] = None
+    rules: Optional[TokenRules] = None
+    rule_set: int = -1                # its place in the engine's RuleStore while it is admitted
+    dropped: int = 0                  # leading blocks that have been looked at for giving back (a model with a window)
     done: threading.Event = field(default_factory=threading.Event)
 
     @property
@@ -126,6 +137,12 @@ class Engine:
         self.cfg = cfg or EngineConfig()
         self.clock = clock
         mcfg: LlamaConfig = model.cfg if model is not None else PRESETS[self.cfg.model]
+        if self.cfg.window < 0 or self.cfg.sinks < 0 or (self.cfg.sinks and not self.cfg.window):
+            raise ValueError(f"window {self.cfg.window}, sinks {self.cfg.sinks}: at least 0, and no sinks without a window")
+        if self.cfg.window and model is None:
+            mcfg = replace(mcfg, window=self.cfg.window, sinks=self.cfg.sinks)
+        elif self.cfg.window and (mcfg.window, mcfg.sinks) != (self.cfg.window, self.cfg.sinks):
+            raise ValueError(f"window {self.cfg.window} + {self.cfg.sinks} sinks for a model of {mcfg.window} + {mcfg.sinks}")
         self.device = torch.device(self.cfg.device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -193,6 +210,10 @@ class Engine:
         self._h_tokens, self._h_i32, self._h_bt = (self._h_tokens_t.numpy(), self._h_i32_t.numpy(),
                                                    self._h_bt_t.numpy())
         self._graphs: Dict[int, object] = {}
+        self._rule_graphs: Dict[int, object] = {}         # the same with rules on the choice
+        self._store: Optional[RuleStore] = None           # made with the first request that has rules
+        self._d_rows: Optional[torch.Tensor] = None       # decode row -> its set of rules
+        self._step_lock = threading.RLock()               # a step, or a change of the cache between two steps
         self._workspace = llm.DecodeWorkspace(B, self.lcfg.n_q, 64, dev) if self.on_gpu else None
 
     # ------------------------------------------------------------------ sizing
@@ -210,10 +231,13 @@ class Engine:
         return self.alloc.total * BLOCK
 
     # ------------------------------------------------------------------ submission
-    def submit(self, prompt: Sequence[int], max_tokens: int = 16) -> Request:
+    def submit(self, prompt: Sequence[int], max_tokens: int = 16, rules: Optional[TokenRules] = None) -> Request:
+        """`rules`: on the choice of this request's tokens (ValueError if they do not fit the vocabulary)."""
+        if rules is not None:
+            rules.check(self.mcfg.vocab)
         now = self.clock()
         with self._lock:
-            r = Request(self._next_id, [int(t) % self.mcfg.vocab for t in prompt], int(max_tokens), now)
+            r = Request(self._next_id, [int(t) % self.mcfg.vocab for t in prompt], int(max_tokens), now, rules=rules)
             self._next_id += 1
             if not r.prompt or r.max_tokens < 1 or len(r.prompt) + 1 > self.max_len or \
                     -(-(len(r.prompt) + 1) // BLOCK) > self.alloc.total:
@@ -265,7 +289,7 @@ class Engine:
         stop_all, n_new = bool(msgs[0][2]), int(msgs[0][3])
         new_specs = []
         if n_new:
-            new_specs = self.tp.broadcast_object([(r.rid, r.prompt, r.max_tokens) for r in new] if self.tp.rank == 0 else None)
+            new_specs = self.tp.broadcast_object([(r.rid, r.prompt, r.max_tokens, *([r.rules] if r.rules else [])) for r in new] if self.tp.rank == 0 else None)
         bad = [i for i, m in enumerate(msgs) if m[0]]
         drift = [i for i, m in enumerate(msgs) if m[1] != msgs[0][1]]
         if bad or drift:
@@ -282,8 +306,8 @@ class Engine:
             if self.tp.rank == 0:
                 self.waiting.extend(new)
             else:
-                for rid, prompt, max_tokens in new_specs:
-                    self.waiting.append(Request(rid, list(prompt), int(max_tokens), now))
+                for rid, prompt, max_tokens, *rules in new_specs:
+                    self.waiting.append(Request(rid, list(prompt), int(max_tokens), now, rules=rules[0] if rules else None))
         return bool(stop_all)
 
     def step_all(self) -> int:
@@ -295,6 +319,10 @@ class Engine:
     # ------------------------------------------------------------------ one iteration
     def step(self) -> int:
         """Run one model launch; returns the number of tokens it produced (0 = nothing to do)."""
+        with self._step_lock:
+            return self._step()
+
+    def _step(self) -> int:
         chunks: List[tuple] = []                    # (request, tokens of it in this launch)
         riders: List[Request] = []                  # running sequences that decode inside a prefill launch
         mixed = self.cfg.mixed_batches
@@ -320,7 +348,7 @@ class Engine:
                     if need > self.alloc.free:
                         break
                     r.blocks = self.alloc.alloc(need)
-                    r.prefilled = 0
+                    r.prefilled = r.dropped = 0
                     self.waiting.popleft()
                     self.prefilling.append(r)
                     take = min(n, budget)
@@ -334,10 +362,44 @@ class Engine:
             return self._decode()
         return 0
 
-    def _finish(self, r: Request, now: float) -> None:
-        r.t_done = now
+    def _let_go(self, r: Request) -> None:
+        """What an admitted request holds goes back: its blocks and its place among the rules."""
         self.alloc.release(r.blocks)
         r.blocks = []
+        if r.rule_set >= 0:
+            self._store.give_back(r.rule_set)
+            r.rule_set = -1
+
+    def _drop_behind(self, r: Request, position: int) -> None:
+        """Give back the blocks that no token from `position` on looks at: those whose last token lies behind its window,
+        unless they hold sinks. Launches are in order on one stream: whoever gets such a block writes it after every read of it."""
+        w = self.mcfg.window
+        if not w:
+            return
+        end = min((position - w + 1) // BLOCK, len(r.blocks))          # blocks below it end at position - window or before
+        first = max(r.dropped, -(-self.mcfg.sinks // BLOCK))
+        if end > first:
+            self.alloc.release(r.blocks[first:end])
+            r.blocks[first:end] = [-1] * (end - first)
+            r.dropped = end
+
+    def _rules_of(self, reqs: Sequence[Request]) -> Optional[List[int]]:
+        """The set of rules that each request of a launch follows (-1: none), their histories brought up to date; None when no
+        request has any."""
+        if all(r.rules is None for r in reqs):
+            return None
+        if self._store is None:
+            self._store = RuleStore(self.cfg.max_num_seqs, self.max_len, self.mcfg.vocab, self.device)
+            self._d_rows = torch.full((self.cfg.max_num_seqs,), -1, dtype=torch.int32, device=self.device)
+        for r in reqs:
+            if r.rules is not None and r.rule_set < 0:
+                r.rule_set = self._store.take(r.rules, len(r.prompt))
+        self._store.follow([(r.rule_set, r.prompt, r.out) for r in reqs if r.rule_set >= 0])
+        return [r.rule_set for r in reqs]
+
+    def _finish(self, r: Request, now: float) -> None:
+        r.t_done = now
+        self._let_go(r)
         self.metrics.on_finish(now - r.arrival)
         r.done.set()
 
@@ -350,7 +412,9 @@ class Engine:
         pos: List[int] = []
         slots: List[int] = []
         info, last_rows = [], []
-        bt = np.zeros((len(chunks), self.max_blocks), dtype=np.int32)
+        # a kernel with a window takes the table's width for the longest context
+        width = max(len(r.blocks) for r, _ in chunks) if self.mcfg.window else self.max_blocks
+        bt = np.zeros((len(chunks), width), dtype=np.int32)
         for i, (r, take) in enumerate(chunks):
             seq = r.prompt + r.out
             lo, hi = r.prefilled, r.prefilled + take
@@ -385,9 +449,11 @@ class Engine:
         meta = PrefillMeta(torch.from_numpy(bt).to(dev), torch.tensor(info, dtype=torch.int32, device=dev),
                            llm.prefill_tiles(q_lens, g, qt, ctx_lens=[c for (_, _, c) in info]).to(dev),
                            torch.tensor(last_rows, dtype=torch.int64, device=dev), qt)
+        sets = self._rules_of([r for r, _ in chunks] + list(riders))
+        kw = {} if sets is None else {"rules": self._store.rules(torch.tensor(sets, dtype=torch.int32, device=dev))}
         nxt = self.model.prefill(torch.tensor(toks, dtype=torch.int64, device=dev),
                                  torch.tensor(pos, dtype=torch.int32, device=dev),
-                                 torch.tensor(slots, dtype=torch.int32, device=dev), self.cache, meta, riders=dmeta)
+                                 torch.tensor(slots, dtype=torch.int32, device=dev), self.cache, meta, riders=dmeta, **kw)
         nxt = nxt.tolist()                      # synchronises
         now = self.clock()
         new_prompt = produced = 0
@@ -396,6 +462,7 @@ class Engine:
                 if r.t_first is None:
                     new_prompt += take
                 r.prefilled += take
+                self._drop_behind(r, r.prefilled)
                 if r.prefilled < r.n_tokens:
                     continue                    # more chunks to go: the sampled token of a partial prompt is dropped
                 self.prefilling.remove(r)
@@ -419,6 +486,8 @@ class Engine:
                 if len(r.out) >= r.max_tokens or r.n_tokens >= self.max_len:
                     self.running.remove(r)
                     self._finish(r, now)
+                else:
+                    self._drop_behind(r, r.n_tokens - 1)
             self.metrics.on_step(produced, new_prompt, len(self.running) + len(self.prefilling), len(self.waiting),
                                  self.alloc.usage)
         kind = "mixed" if riders else "prefill"
@@ -439,8 +508,7 @@ class Engine:
             if self.alloc.free == 0:
                 # most recently admitted first: a request still in prefill loses the least work
                 victim = self.prefilling.pop() if self.prefilling else self.running.pop()
-                self.alloc.release(victim.blocks)
-                victim.blocks = []
+                self._let_go(victim)
                 victim.prefilled = 0
                 victim.preempted += 1
                 self.waiting.appendleft(victim)
@@ -471,11 +539,14 @@ class Engine:
             hv[1, i] = r.blocks[(nt - 1) // BLOCK] * BLOCK + (nt - 1) % BLOCK
             hv[2, i] = nt
             hb[i, :len(r.blocks)] = r.blocks
+        sets = self._rules_of(seqs)
+        if sets is not None:
+            self._d_rows[:b].copy_(torch.tensor(sets + [-1] * (b - n), dtype=torch.int32))
         # the pinned host buffers are not touched again before the .tolist() below has synchronised
         self._d_tokens[:b].copy_(self._h_tokens_t[:b], non_blocking=True)
         self._d_i32.copy_(self._h_i32_t, non_blocking=True)
         self._d_bt[:b].copy_(self._h_bt_t[:b], non_blocking=True)
-        self._run_decode(b)
+        self._run_decode(b, sets is not None)
         nxt = self._d_next[:n].tolist()         # synchronises
         now = self.clock()
         with self._lock:
@@ -487,6 +558,7 @@ class Engine:
                 if len(r.out) >= r.max_tokens or r.n_tokens >= self.max_len:
                     self._finish(r, now)
                 else:
+                    self._drop_behind(r, r.n_tokens - 1)
                     still.append(r)
             self.running = still
             self.metrics.on_step(n, 0, len(self.running) + len(self.prefilling), len(self.waiting), self.alloc.usage)
@@ -495,30 +567,32 @@ class Engine:
         self.step_log.append((t0, now - t0, "decode", n, n))
         return n
 
-    def _decode_call(self, b: int) -> None:
+    def _decode_call(self, b: int, ruled: bool = False) -> None:
         meta = DecodeMeta(self._d_bt[:b], self._d_ctx[:b],
                           num_splits=llm.pick_splits(b, self.lcfg.n_kv, self.max_len) if self.on_gpu else 1,
                           workspace=self._workspace)
-        out = self.model.decode(self._d_tokens[:b], self._d_pos[:b], self._d_slots[:b], self.cache, meta)
+        kw = {"rules": self._store.rules(self._d_rows[:b])} if ruled else {}
+        out = self.model.decode(self._d_tokens[:b], self._d_pos[:b], self._d_slots[:b], self.cache, meta, **kw)
         self._d_next[:b].copy_(out)
 
-    def _run_decode(self, b: int) -> None:
+    def _run_decode(self, b: int, ruled: bool = False) -> None:
         if not (self.on_gpu and self.cfg.use_graphs):
-            self._decode_call(b)
+            self._decode_call(b, ruled)
             return
-        g = self._graphs.get(b)
+        graphs = self._rule_graphs if ruled else self._graphs
+        g = graphs.get(b)
         if g is None:
             # warm up on a side stream (library handles, allocator pools), then capture
             s = torch.cuda.Stream(self.device)
             s.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(s):
-                self._decode_call(b)
+                self._decode_call(b, ruled)
             torch.cuda.current_stream(self.device).wait_stream(s)
             torch.cuda.synchronize(self.device)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                self._decode_call(b)
-            self._graphs[b] = g
+                self._decode_call(b, ruled)
+            graphs[b] = g
         g.replay()
 
     def warmup(self, buckets: Optional[Sequence[int]] = None) -> None:
@@ -530,6 +604,31 @@ class Engine:
         for b in (buckets or self.buckets):
             self._run_decode(b)
         torch.cuda.synchronize(self.device)
+
+    def resize_cache(self, num_blocks: int) -> None:
+        """Another number of cache blocks, between two steps: the blocks in use move to the front of a new cache and the old one's
+        memory goes back (both exist while they move). Captured graphs read the old addresses and are captured again when
+        needed. ValueError where the blocks would not hold what is in flight, or a request that waits, to its end."""
+        if self.tp.world > 1:
+            raise ValueError("resize_cache: the ranks of a tensor-parallel engine take the smallest count when they start")
+        with self._step_lock, self._lock:
+            live = self.prefilling + self.running
+            held = sum(1 for r in live for b in r.blocks if b >= 0)
+            most = max((-(-(len(r.prompt) + r.max_tokens) // BLOCK) for r in [*live, *self.waiting]), default=1)
+            if num_blocks < max(held, most):
+                raise ValueError(f"resize_cache: {num_blocks} blocks; {held} are in use and a request may come to {most}")
+            cache, old = self.model.new_cache(num_blocks, self.kv_dtype), self.cache
+            alloc = BlockAllocator(num_blocks)
+            to = dict(zip((b for r in live for b in r.blocks if b >= 0), alloc.alloc(held)))
+            llm.copy_pages(cache.k, cache.v, list(to.items()), k_src=old.k, v_src=old.v)
+            for r in live:
+                r.blocks = [to.get(b, -1) for b in r.blocks]
+            if self.on_gpu:
+                torch.cuda.synchronize(self.device)       # the graphs' last run and the copies end before what they use goes
+            self._graphs.clear()
+            self._rule_graphs.clear()
+            self.cache, self.alloc = cache, alloc
+            self.metrics.set_queue(len(self.running), len(self.waiting), alloc.usage)
 
     # ------------------------------------------------------------------ background loop
     def start(self) -> "Engine":
@@ -574,9 +673,7 @@ class Engine:
         now = self.clock()
         with self._lock:
             for r in list(self._inbox) + list(self.waiting) + list(self.prefilling) + list(self.running):
-                if r.blocks:
-                    self.alloc.release(r.blocks)
-                r.blocks = []
+                self._let_go(r)
                 r.error = why
                 r.t_done = now
                 r.done.set()
@@ -616,10 +713,11 @@ class Engine:
                 "kv_bytes": self.cache.nbytes, "max_num_seqs": self.cfg.max_num_seqs, "max_model_len": self.max_len,
                 "graphs": sorted(self._graphs), "device": str(self.device),
                 "decode_weights": "fp8 (W8A16, batch <= 128)" if self.model.fp8_decode else "bf16",
+                "window": self.mcfg.window, "sinks": self.mcfg.sinks,
                 "kv_cache_dtype": self.cfg.kv_cache_dtype, "mixed_batches": self.cfg.mixed_batches,
                 # which kernels a launch of n rows runs on (rows outside these ranges: hipBLASLt + separate norm / rope / SwiGLU)
                 "kernel_paths": {"skinny_rows": self.model.skinny_rows(), "mid_spans": [list(x) for x in self.model.mid_spans()],
-                                 "fused_rope_attention": bool(self.model.fused_rope and self.on_gpu and self.kv_dtype is None)},
+                                 "fused_rope_attention": bool(self.model.fused_rope and self.on_gpu and self.kv_dtype is None and not self.mcfg.window)},
                 "max_num_batched_tokens": self.cfg.max_num_batched_tokens,
                 "step_seconds": dict(self.step_seconds), "step_counts": dict(self.step_counts),
                 "tensor_parallel": self.tp.describe(), "errors": self.errors, "last_error": self.last_error}

@@ -3,7 +3,8 @@
     GET  /metrics            Prometheus text with vLLM's metric names (scraped by collectors/vllm.py)
     GET  /health             200 once the engine thread runs
     GET  /v1/models          the served model
-    POST /v1/completions     {"prompt": [token ids] | "prompt_len": n, "max_tokens": m} -> token ids
+    POST /v1/completions     {"prompt": [token ids] | "prompt_len": n, "max_tokens": m} -> token ids; optional rules on the choice:
+                             repetition_penalty, frequency_penalty, presence_penalty, logit_bias, allowed_token_ids
     GET  /stats[?window=S]   exact ground truth (quantiles, rates) + engine description
     GET  /trace              the recent model launches as a Chrome trace (open in Perfetto)
 
@@ -20,6 +21,7 @@ from http.server import BaseHTTPRequestHandler, ThreadingHTTPServer
 from typing import Optional
 
 from .engine import Engine
+from .rules import TokenRules
 
 
 class LlmServer:
@@ -94,10 +96,11 @@ class LlmServer:
                     max_tokens = int(req.get("max_tokens") or 16)
                     if not 1 <= max_tokens <= outer.engine.max_len:
                         raise ValueError(f"max_tokens must be within 1..{outer.engine.max_len}")
+                    rules = TokenRules.from_request(req, outer.engine.mcfg.vocab)
                 except (ValueError, TypeError, json.JSONDecodeError) as e:
                     self._json(400, {"error": str(e)})
                     return
-                r = outer.engine.submit(ids, max_tokens)
+                r = outer.engine.submit(ids, max_tokens, rules) if rules is not None else outer.engine.submit(ids, max_tokens)
                 if not r.done.wait(outer.request_timeout):
                     self._json(504, {"error": "timed out", "id": r.rid})
                     return

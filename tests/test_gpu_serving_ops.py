@@ -144,6 +144,16 @@ def test_a_bad_value_reaches_only_the_rows_that_see_it(dtype, bad):
     _near(got[~hit], want[~hit], size[~hit])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("kind,seqs,n_q,n_kv,window,sinks", [("decode", DECODE, 20, 1, 50, 4), ("prefill", PREFILL, 8, 2, 50, 4), ("prefill", [(0, 300, 900)], 16, 2, 200, 3),
+                                                             ("prefill", [(0, 1300, 2000)], 64, 8, 300, 20)])
+def test_what_masked_places_hold_moves_no_bit(dtype, kind, seqs, n_q, n_kv, window, sinks):
+    """NaN or 0 in every place that no row sees: not a value of the result may differ, whichever way the kernel took."""
+    call = _decode if kind == "decode" else _prefill
+    got = [call(*make(kind, seqs, n_q, n_kv, window, sinks, dtype, poison=p), seqs, n_q, window, sinks) for p in (True, False)]
+    assert bool(torch.isfinite(got[0]).all()) and torch.equal(*got)
+
+
 def test_large_scores_and_a_growing_maximum():
     """Scores in the hundreds, each key's larger than the one before it: the running maximum moves at every step."""
     for kind, seqs in (("decode", [150, 40]), ("prefill", [(0, 150, 150), (150, 40, 90)])):
