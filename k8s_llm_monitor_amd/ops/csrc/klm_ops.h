@@ -195,7 +195,7 @@ typedef struct klm_window_args {
   float *part_o, *part_ml;
   void* stream;
   int n_seqs, rows, q_stride, n_q, n_kv, width, pages, window, sinks, splits, kv_fp8;
-  int q_tiles;                       // prefill: 16-row query tiles of a wave, 1 or 3
+  int q_tiles;                       // prefill: 16-row query tiles of a wave, 1 or 2
   int zero_rest;                     // prefill: rows of no sequence become 0 (else they are not written)
   float scale;
 } klm_window_args;

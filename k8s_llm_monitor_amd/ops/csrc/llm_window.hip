@@ -272,29 +272,32 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(WinArgs a, int he
 // decode's (and llm_attention.hip's): lane (fr, fq) has query row fr and, after S^T = K Q^T, the scores of keys fq*8 .. + 7;
 // these are the second operand that O^T = V^T P wants from it, no value changes lanes.
 // LDS step: K [32 tokens][16 chunks of 16 bytes], chunk c of token t at c ^ key(t): the 16 rows of a fragment read 16 chunk
-// columns. V [page][dims/16][half][dims%16] chunks of 8 tokens: half a wave reads 512 bytes in lane order. A ring of 4 steps; a bf16 cache is
-// brought in by LDS-DMA three steps ahead (4 KiB a wave, no registers), an e4m3 cache through registers, where it becomes
-// bf16 once per block.
+// columns. V [page][dims/16][half][dims%16] chunks of 8 tokens: half a wave reads 512 bytes in lane order. Two steps of each: while
+// one is worked on the next is brought in, a bf16 cache by LDS-DMA (4 KiB a wave, no registers), an e4m3 cache by LDS-DMA as it
+// is and turned into bf16 once per block.
+// What bounds it: a step of two tiles is 32 matrix instructions (512 clocks) and 80 vector ones, 16 of them exp2 (400); with three
+// waves a SIMD they fill 55 and 45 % of the time, the rest waits on LDS and the barrier. Two tiles, because they and their state
+// fit 168 registers, three blocks a CU; three tiles at two blocks a CU, with the scores of a step computed under the weights of
+// the one before, took 391 us where this takes 384 (8192 tokens, 32 heads over 8, window 4096: 1075 TFLOP/s) and 293 where this
+// takes 260 (e4m3, chunks of a long context). One tile for fewer rows: 128 registers, four blocks a CU. A third step in LDS, wave
+// priorities and sums by matrix instructions gave nothing.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int STEP_BYTES = 16384, RING = 4;
+constexpr int HALF = 8192;      // a step's K, or its V, in LDS
 
 __device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) & 3) << 2); }
 
 #define KLM_AS3 __attribute__((address_space(3)))
-struct Pages2 {
-  int p0, p1;            // a step's two pages, -1: none
-};
 
 // A wave brings a quarter of a step, half a page: K tokens 8w .. 8w + 7 (the chunk swizzle is the same for both fours of
-// them), V dims 64 (w % 2) .. + 63; `ko`, `vo`: the lane's offsets in bytes inside the page. The second half of each lies 1 KiB
+// them), V dims 64 (w % 2) .. + 63; `at`: number of the page's block of this kv head in the cache, -1: none; `ko`, `vo`: the lane's
+// offsets in bytes inside it. The second half of each lies 1 KiB
 // behind the first, in memory as in LDS.
 // Written in assembly because the compiler takes the builtin for an access that may hit LDS at any time, and then waits for all
 // outstanding LDS reads at each of them (and for the DMA before them); what has landed is said by the kernel's own waits. No
 // register is written but m0, which nothing else here uses. s_nop 4: a scalar base that a vector instruction wrote may be
 // read by a memory instruction five states later; s_nop 0: m0 before its use.
-__device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, uint32_t st, int w, unsigned ko, unsigned vo) {
-  const int id = w < 2 ? pg.p0 : pg.p1;
-  const size_t base = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * (BLK_ELEMS * 2);
+__device__ __forceinline__ void dma_step(const WinArgs& a, int at, uint32_t st, int w, unsigned ko, unsigned vo) {
+  const size_t base = (size_t)(at < 0 ? 0 : at) * (BLK_ELEMS * 2);
   const char* k = (const char*)a.kc + base;
   const char* v = (const char*)a.vc + base;
   asm volatile(
@@ -307,15 +310,14 @@ __device__ __forceinline__ void dma_step(const WinArgs& a, Pages2 pg, int h, uin
       "global_load_lds_dwordx4 %1, %3\n\t"
       "global_load_lds_dwordx4 %1, %3 offset:1024"
       :
-      : "v"(ko), "v"(vo), "s"(k), "s"(v), "s"(st + w * 2048), "s"(st + 8192 + w * 2048)
+      : "v"(ko), "v"(vo), "s"(k), "s"(v), "s"(st + w * 2048), "s"(st + 2 * HALF + w * 2048)
       : "memory");
 }
 
 // The same of an e4m3 cache: a wave's 2 KiB of raw bytes go to a corner of its own, `raw`, from where it turns them into the bf16
 // step one step later. A lane's 16 bytes: 16 dims of a key, 16 tokens of a dim.
-__device__ __forceinline__ void dma_step8(const WinArgs& a, Pages2 pg, int h, uint32_t raw, int w, unsigned off) {
-  const int id = w < 2 ? pg.p0 : pg.p1;
-  const size_t base = ((size_t)(id < 0 ? 0 : id) * a.n_kv + h) * BLK_ELEMS + (w & 1) * 1024;
+__device__ __forceinline__ void dma_step8(const WinArgs& a, int at, uint32_t raw, int w, unsigned off) {
+  const size_t base = (size_t)(at < 0 ? 0 : at) * BLK_ELEMS + (w & 1) * 1024;
   const char* k = (const char*)a.kc + base;
   const char* v = (const char*)a.vc + base;
   asm volatile(
@@ -336,7 +338,7 @@ __device__ __forceinline__ void widen_step8(char* st, const char* raw, int w, in
   *reinterpret_cast<bf16x8*>(kp + ((c ^ key) << 4)) = fp8x8_to_bf16(k.x, k.y);
   *reinterpret_cast<bf16x8*>(kp + (((c + 1) ^ key) << 4)) = fp8x8_to_bf16(k.z, k.w);
   const int dim = (w & 1) * 64 + lane;
-  char* vp = st + 8192 + (w >> 1) * 4096 + (dim >> 4) * 512 + (dim & 15) * 16;
+  char* vp = st + 2 * HALF + (w >> 1) * 4096 + (dim >> 4) * 512 + (dim & 15) * 16;
   *reinterpret_cast<bf16x8*>(vp) = fp8x8_to_bf16(v.x, v.y);
   *reinterpret_cast<bf16x8*>(vp + 256) = fp8x8_to_bf16(v.z, v.w);
 }
@@ -435,70 +437,37 @@ __device__ __forceinline__ uint32_t odd_marks(uint32_t x) {
   return r;
 }
 
-// What a wave does with one 32-key step, in two parts, so that matrix and vector instructions of different steps can run at the
-// same time: while the scores of step i + 1 are multiplied, the weights of step i are taken from their exponents (part A); while
-// step i's weights meet V, step i + 1's scores become exponents (part B).
+// The weights of a tile's exponents. The sum is taken of the weights as they are, V meets them rounded to bf16 (half a step, 2^-9,
+// of each, as often up as down).
 template <int QT>
-struct Scores {
-  f32x4 s[QT][2];
-};
-
-// Weights 2 c and 2 c + 1 of tile t's exponents. The sum is taken of the rounded weights, two at a time: they are what meets V.
-template <int QT>
-__device__ __forceinline__ void weights(Rows<QT>& r, const float (&x)[QT][8], int t, int c, bf16x8& p) {
-  const bf16x2 two = bf16x2{(__bf16)fast_exp2(x[t][2 * c]), (__bf16)fast_exp2(x[t][2 * c + 1])};
-  p[2 * c] = two[0];
-  p[2 * c + 1] = two[1];
-  r.l[t] = __builtin_amdgcn_fdot2_f32_bf16(two, bf16x2{(__bf16)1.f, (__bf16)1.f}, r.l[t], false);
-}
-
-template <int QT>
-__device__ __forceinline__ void part_a(const char* st, int lane, Rows<QT>& r, const float (&x)[QT][8], Scores<QT>& s, bf16x8 (&p)[QT]) {
-  const int fr = lane & 15, fq = lane >> 4;
-  const char* kp = st + ((fr >> 2) * 8 + (fr & 3)) * 256;              // k_key of both tokens below is fr
+__device__ __forceinline__ void weights(Rows<QT>& r, const float (&x)[QT][8], int t, bf16x8& p) {
 #pragma unroll
-  for (int t = 0; t < QT; ++t) s.s[t][0] = s.s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
-    const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      s.s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s.s[t][0], 0, 0, 0);
-      s.s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s.s[t][1], 0, 0, 0);
-      weights<QT>(r, x, t, c, p[t]);
-    }
+  for (int j = 0; j < 8; j += 2) {
+    const float e0 = fast_exp2(x[t][j]), e1 = fast_exp2(x[t][j + 1]);
+    p[j] = (__bf16)e0;
+    p[j + 1] = (__bf16)e1;
+    r.l[t] += e0 + e1;
   }
 }
 
-template <int QT>
-__device__ __forceinline__ void part_b(const WinArgs& a, const char* st, int lane, Rows<QT>& r, const Scores<QT>& s, const bf16x8 (&p)[QT],
-                                       float (&x)[QT][8], float (&mx)[QT]) {
-  const int fq = lane >> 4;
-  const char* vp = st + 8192 + (fq >> 1) * 4096 + (lane & 31) * 16;
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 512);
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
-      x[t][n] = fmaf(n < 4 ? s.s[t][0][n & 3] : s.s[t][1][n & 3], a.scale_log2, r.shift[t]);
-      mx[t] = n ? fmaxf(mx[t], x[t][n]) : x[t][n];
-    }
-  }
+// bit j: the row at `pos` sees key + j, j = 0 .. 7
+__device__ __forceinline__ uint32_t seen_bits(const WinArgs& a, int pos, int key) {
+  const auto below = [](int n) { return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1; };         // bits 0 .. n - 1
+  return below(pos - key + 1) & (~below(pos - key - a.window + 1) | below(a.sinks - key));
 }
 
-// Masks the exponents of a step that some row does not see whole.
+// Masks the exponents of a step that some row does not see whole; bit i of `pages`: its page i is there.
 template <int QT>
-__device__ __forceinline__ void mask_step(const WinArgs& a, int step, Pages2 pg, int lane, const Rows<QT>& r, float (&x)[QT][8], float (&mx)[QT]) {
+__device__ __forceinline__ void mask_step(const WinArgs& a, int step, int pages, int lane, const Rows<QT>& r, float (&x)[QT][8], float (&mx)[QT]) {
   const int fq = lane >> 4, key = step * 32 + fq * 8;                  // the lane's scores: keys key .. + 7, of one page
-  const bool page = ((fq >> 1) ? pg.p1 : pg.p0) >= 0;
+  const bool page = (pages >> (fq >> 1)) & 1;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const int up = page ? r.pos[t] - key : -1, down = r.pos[t] - key - a.window, sink = a.sinks - key;
+    const uint32_t see = page ? seen_bits(a, r.pos[t], key) : 0u;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[t][j] = j <= up && (j > down || j < sink) ? x[t][j] : -INFINITY;
+      const uint32_t all = (uint32_t)((int)(see << (31 - j)) >> 31);
+      x[t][j] = __uint_as_float((all & __float_as_uint(x[t][j])) | (~all & 0xff800000u));        // -inf where the bit is not set
       mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
     }
   }
@@ -528,19 +497,6 @@ __device__ __forceinline__ void move_maximum(Rows<QT>& r, float (&x)[QT][8], flo
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[t][j] -= by;
   }
-}
-
-// A row that does not see a key has weight 0 for it, and 0 times a NaN or an infinity in V would be NaN: a step at the edge that
-// holds such values sends the wave's rows to careful_tile.
-__device__ __forceinline__ bool odd_values(const char* st, int lane) {
-  const char* vp = st + 8192 + lane * 16;
-  uint32_t any = 0;
-#pragma unroll 2                                                       // not more: registers
-  for (int n = 0; n < 8; ++n) {
-    const uint4 u = *reinterpret_cast<const uint4*>(vp + n * 1024);
-    any |= odd_halves(u.x) | odd_halves(u.y) | odd_halves(u.z) | odd_halves(u.w);
-  }
-  return __ballot(any != 0) != 0;
 }
 
 // The finished rows of one 16-row tile: lane (fr, fq) holds dims n * 16 + fq * 4 .. + 3 of row fr; dst < 0: no row.
@@ -576,9 +532,10 @@ __device__ __forceinline__ bf16x8 load8(const void* cache, size_t at) {
   return *reinterpret_cast<const bf16x8*>((const uint16_t*)cache + at);
 }
 
-// One 16-row tile again, from the cache and by themselves, where V holds NaN or infinities that some rows see and others do not:
-// they leave the matrix product, and the rows that see them get them back. Rare and slow: one step after another, every load
-// waited for. Each number is made as the fast loop makes it, so what a masked place holds does not move a single bit.
+// One 16-row tile again, from the cache and by itself, where V holds NaN or infinities that some rows see and others do not (a
+// weight of 0 times them is NaN): they leave the matrix product, and the rows that see them get them back. Rare and slow: one
+// step after another, every load waited for. Each number is made as the fast loop makes it, so what a masked place holds does not
+// move a single bit.
 template <bool KV8, typename Inside>
 __device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table, int h, const Span& sp, int i0, int i1, int split, int lane,
                                              const uint16_t* qrow, int pos, int64_t dst, const Inside& is_inside) {
@@ -599,8 +556,9 @@ __device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table,
 #pragma unroll 1
   for (int i = i0; i < i1; ++i) {
     const int step = sp.step(i), key = step * 32 + fq * 8;
-    const Pages2 pg{page_at(table, step * 2, a.width, a.pages), page_at(table, step * 2 + 1, a.width, a.pages)};
-    const size_t b0 = ((size_t)(pg.p0 < 0 ? 0 : pg.p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(pg.p1 < 0 ? 0 : pg.p1) * a.n_kv + h) * BLK_ELEMS;
+    const int p0 = page_at(table, step * 2, a.width, a.pages), p1 = page_at(table, step * 2 + 1, a.width, a.pages);
+    const int pages = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+    const size_t b0 = ((size_t)(p0 < 0 ? 0 : p0) * a.n_kv + h) * BLK_ELEMS, b1 = ((size_t)(p1 < 0 ? 0 : p1) * a.n_kv + h) * BLK_ELEMS;
     const size_t ko = ((fr >> 3) ? b1 : b0) + ((((fr >> 2) & 1) << 3) + (fr & 3)) * HD + fq * 8;
     const size_t vo = ((fq >> 1) ? b1 : b0) + fr * BLK + (fq & 1) * 8;
     f32x4 s0 = f32x4{0.f, 0.f, 0.f, 0.f}, s1 = s0;
@@ -613,16 +571,15 @@ __device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table,
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[0][j] = fmaf(j < 4 ? s0[j & 3] : s1[j & 3], a.scale_log2, r.shift[0]);
     mx[0] = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[0][4], x[0][5]), fmaxf(x[0][6], x[0][7])));
-    if (!is_inside(step, pg)) mask_step<1>(a, step, pg, lane, r, x, mx);
+    if (!is_inside(i, pages)) mask_step<1>(a, step, pages, lane, r, x, mx);
     move_maximum<1>(r, x, mx);
-    const int up = ((fq >> 1) ? pg.p1 : pg.p0) >= 0 ? pos - key : -1, down = pos - key - a.window, sink = a.sinks - key;
+    const uint32_t see = (pages >> (fq >> 1)) & 1 ? seen_bits(a, pos, key) : 0u;
     bf16x8 p;
     uint32_t ones[4] = {0u, 0u, 0u, 0u};                               // 1 for a key that the row sees, as bf16 pairs
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ones[j >> 1] |= j <= up && (j > down || j < sink) ? 0x3f80u << (16 * (j & 1)) : 0u;
+    for (int j = 0; j < 8; ++j) ones[j >> 1] |= ((see >> j) & 1) * 0x3f80u << (16 * (j & 1));
     const bf16x8 one = __builtin_bit_cast(bf16x8, uint4{ones[0], ones[1], ones[2], ones[3]});
-#pragma unroll
-    for (int c = 0; c < 4; ++c) weights<1>(r, x, 0, c, p);
+    weights<1>(r, x, 0, p);
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const uint4 u = __builtin_bit_cast(uint4, load8<KV8>(a.vc, vo + n * 16 * BLK));
@@ -644,7 +601,7 @@ __device__ __forceinline__ void careful_tile(const WinArgs& a, const int* table,
 }
 
 template <int QT, bool KV8>
-__global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, QT == 1 && !KV8 ? 4 : 3) void window_prefill_kernel(WinArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int h = blockIdx.x, split = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -699,130 +656,117 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     r.l[t] = 0.f;
   }
 
-  // does every row of the wave see all of a step? (Rows that are none see what they like then: they are not written.)
-  const auto is_inside = [&](int step, Pages2 pg) {
-    const int k0 = step * 32;
-    return k0 + 31 <= pmin && (k0 > pmax - a.window || k0 + 31 < a.sinks) && pg.p0 >= 0 && pg.p1 >= 0;
+  // Does every row of the wave see all of step i? (Rows that are none see what they like then: they are not written.) Of the sinks'
+  // steps the first `in_sinks`, of the window's those from in_a to in_b.
+  const int whole = (pmin + 1) >> 5, in_sinks = (a.sinks >> 5) < whole ? (a.sinks >> 5) : whole;
+  const int in_a = (pmax < a.window ? 0 : ((pmax - a.window) >> 5) + 1) - sp.lo_step + sp.n_sink, in_b = whole - sp.lo_step + sp.n_sink;
+  const auto is_inside = [&](int i, int pages) {
+    return pages == 3 && (i < sp.n_sink ? i < in_sinks : i >= in_a && i < in_b);
   };
-  bool odd = false;
+  const bool nobody = ta >= q_len;                                     // the wave has no rows: it brings its part of the cache and no more
   if (i0 < i1) {
     const int last = i1 - 1;
     const int tok = w * 8 + (lane >> 4);
     const unsigned ko = (tok & 15) * 256 + (((lane & 15) ^ k_key(tok)) << 4);
     const unsigned vo = ((w & 1) * 64 + (lane >> 5) * 16 + (lane & 15)) * 32 + ((lane >> 4) & 1) * 16;
-    const auto step_of = [&](int i) { return sp.step(i < last ? i : last); };      // past the last step: that one again, unused
-    // Pages of step i + 1, i + 2 and i + 3. At step i its V and the K of i + 1 are in LDS, i + 2 is on its way, and i + 3 takes the
-    // place of i - 1, which all waves have left at the barrier.
     // The table's entries for 32 steps at a time lie in one register, a lane each: looking them up in the loop through the scalar
-    // cache would share the LDS reads' counter and make every wait on them a wait for all of them.
+    // cache would share the LDS reads' counter and make every wait on them a wait for all of them. They are numbers of this kv
+    // head's blocks in the cache, -1: no page. `there`: which of them are pages.
     int held;
-    const auto hold = [&](int i) {                                     // steps i .. i + 31
-      const int e = step_of(i + (lane >> 1)) * 2 + (lane & 1);
+    uint64_t there;
+    const auto hold = [&](int i) {                                     // steps i .. i + 31; past the last step: that one again, unused
+      const int at = i + (lane >> 1), e = sp.step(at < last ? at : last) * 2 + (lane & 1);
       const int id = table[e < a.width ? e : a.width - 1];
-      held = e < a.width && (unsigned)id < (unsigned)a.pages ? id : -1;
+      held = e < a.width && (unsigned)id < (unsigned)a.pages ? id * a.n_kv + h : -1;
+      there = __ballot(held >= 0);
     };
-    const auto pages_at = [&](int i) {                                 // of step i0 + i, i in the 32 that are held
-      return Pages2{__builtin_amdgcn_readlane(held, (i & 31) * 2), __builtin_amdgcn_readlane(held, (i & 31) * 2 + 1)};
-    };
+    const auto mine_at = [&](int at) { return __builtin_amdgcn_readlane(held, (at & 31) * 2 + (w >> 1)); };       // what this wave brings of step i0 + at
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((KLM_AS3 char*)lds);
+    // e4m3: two raw corners a wave behind the bf16 steps; step i + 1 is widened at step i, while i + 2 lands in the other corner
+    const uint32_t raw0 = lds0 + 4 * HALF + w * 2048;
+    const char* const raws = lds + 4 * HALF + w * 2048;
     hold(i0);
-    const Pages2 now = pages_at(0);
-    Pages2 next = pages_at(1), after = pages_at(2), far = pages_at(3);
-    // e4m3: two raw corners a wave behind the ring. Step i + 2 is widened at step i, while i + 3 lands in the other corner.
-    const uint32_t raw0 = lds0 + RING * STEP_BYTES + w * 2048;
-    char* const raws = lds + RING * STEP_BYTES + w * 2048;
-    const unsigned off = lane * 16;
     if (KV8) {
-      dma_step8(a, now, h, raw0, w, off);
-      dma_step8(a, next, h, raw0 + 8192, w, off);
+      dma_step8(a, mine_at(0), raw0, w, lane * 16);
+      dma_step8(a, mine_at(1), raw0 + HALF, w, lane * 16);
       asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
       widen_step8(lds, raws, w, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // the corner has been read
-      dma_step8(a, after, h, raw0, w, off);
-      asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-      widen_step8(lds + STEP_BYTES, raws + 8192, w, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
-      dma_step(a, now, h, lds0, w, ko, vo);
-      dma_step(a, next, h, lds0 + STEP_BYTES, w, ko, vo);
-      dma_step(a, after, h, lds0 + 2 * STEP_BYTES, w, ko, vo);
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      dma_step(a, mine_at(0), lds0, w, ko, vo);
     }
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    float x[QT][8], mx[QT];
-    bf16x8 p[QT];
-    bool inside = is_inside(sp.step(i0), now);
-    {
-      Scores<QT> s;
-      const char* kp = lds + ((fr >> 2) * 8 + (fr & 3)) * 256;
-#pragma unroll
-      for (int t = 0; t < QT; ++t) s.s[t][0] = s.s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
-        const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          s.s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s.s[t][0], 0, 0, 0);
-          s.s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s.s[t][1], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[t][j] = fmaf(j < 4 ? s.s[t][0][j & 3] : s.s[t][1][j & 3], a.scale_log2, r.shift[t]);
-          mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
-        }
-    }
-    if (!inside) mask_step<QT>(a, sp.step(i0), now, lane, r, x, mx);
-    move_maximum<QT>(r, x, mx);
+    uint64_t pages = there;                                            // the step's two in its lowest bits
     for (int i = i0; i < i1; ++i) {
-      const int at = i - i0;
+      const int at = i - i0, cur = (at & 1) * HALF, other = HALF - cur;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // what was brought, and widened, during the last step
+      __builtin_amdgcn_s_barrier();                                    // ... by all waves, and all have left the step before
+      asm volatile("" ::: "memory");
+      const int now = pages & 3;
+      pages >>= 2;
       if (KV8) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the raw step i + 2 has landed, this wave's part of i + 1 is written
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        dma_step8(a, far, h, raw0 + ((at + 1) & 1) * 8192, w, off);    // read for the last time one step ago
-        widen_step8(lds + ((at + 2) & (RING - 1)) * STEP_BYTES, raws + (at & 1) * 8192, w, lane);
+        if (((at + 1) & 31) == 0) pages = there;                       // (held one step ago)
+        if (((at + 2) & 31) == 0) hold(i + 2);
+        dma_step8(a, mine_at(at + 2), raw0 + cur, w, lane * 16);       // the corner was read one step ago
+        widen_step8(lds + other, raws + other, w, lane);
       } else {
-        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");               // 4 DMA instructions a wave and step, in order: i + 1 has landed
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        dma_step(a, far, h, lds0 + ((at + 3) & (RING - 1)) * STEP_BYTES, w, ko, vo);
+        if (((at + 1) & 31) == 0) {
+          hold(i + 1);
+          pages = there;
+        }
+        dma_step(a, mine_at(at + 1), lds0 + other, w, ko, vo);
       }
-      const char* st = lds + (at & (RING - 1)) * STEP_BYTES;
-      const char* st1 = lds + ((at + 1) & (RING - 1)) * STEP_BYTES;
-      const int step1 = step_of(i + 1);
-      const bool inside1 = is_inside(step1, next);
-      const Pages2 pg1 = next;
-      next = after;
-      after = far;
-      if (((at + 4) & 31) == 0) hold(i + 4);
-      far = pages_at(at + 4);
-      if (!inside) odd = odd || odd_values(st, lane);
-      Scores<QT> s;
-      part_a<QT>(st1, lane, r, x, s, p);
-      part_b<QT>(a, st, lane, r, s, p, x, mx);
-      if (!inside1) mask_step<QT>(a, step1, pg1, lane, r, x, mx);
+      if (nobody) continue;
+      const char* kp = lds + cur + ((fr >> 2) * 8 + (fr & 3)) * 256;   // k_key of both tokens below is fr
+      const char* vst = lds + 2 * HALF + cur;
+      const bool inside = is_inside(i, now);
+      float x[QT][8], mx[QT];
+      {
+        f32x4 s[QT][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(kp + (((c * 4 + fq) ^ fr) << 4));
+          const bf16x8 k1 = *reinterpret_cast<const bf16x8*>(kp + 1024 + (((c * 4 + fq) ^ fr) << 4));
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, r.q[t][c], s[t][0], 0, 0, 0);
+            s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, r.q[t][c], s[t][1], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[t][j] = fmaf(j < 4 ? s[t][0][j & 3] : s[t][1][j & 3], a.scale_log2, r.shift[t]);
+            mx[t] = j ? fmaxf(mx[t], x[t][j]) : x[t][j];
+          }
+      }
+      if (!inside) mask_step<QT>(a, sp.step(i), now, lane, r, x, mx);
       move_maximum<QT>(r, x, mx);
-      inside = inside1;
+      bf16x8 p[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) weights<QT>(r, x, t, p[t]);
+      const char* vp = vst + (fq >> 1) * 4096 + (lane & 31) * 16;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const bf16x8 v = *reinterpret_cast<const bf16x8*>(vp + n * 512);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) r.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], r.o[t][n], 0, 0, 0);
+      }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // the last, unused steps land before the LDS goes away
   }
 
-  if (odd) {
-#pragma unroll 1
-    for (int t = 0; t < QT; ++t) {
-      int token, g;
-      row_of(t, token, g);
-      const bool valid = token < q_len;
-      const size_t row = q_start + (valid ? token : 0), head = (size_t)h * G + g;
-      careful_tile<KV8>(a, table, h, sp, i0, i1, split, lane, a.q + row * a.q_stride + head * HD, valid ? first + token : -1,
-                        valid ? (int64_t)(row * a.n_q + head) : -1, is_inside);
-    }
-    return;
+  // a NaN in a row's sums: was it the row's to see?
+  unsigned odd = 0;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float any = 0.f;
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) any = fmaf(r.o[t][n][j], 0.f, any);
+    odd |= __ballot(r.pos[t] >= 0 && any != 0.f) ? 1u << t : 0u;
   }
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -830,7 +774,17 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WinArgs a) {
     r.l[t] += __shfl_xor(r.l[t], 32);
     int token, g;
     row_of(t, token, g);
-    write_rows(a, token < q_len ? (int64_t)((size_t)(q_start + token) * a.n_q + (size_t)h * G + g) : -1, split, fq, r.o[t], r.lim[t] > 0.f ? -r.shift[t] : -INFINITY, r.l[t]);
+    const int64_t dst = token < q_len ? (int64_t)((size_t)(q_start + token) * a.n_q + (size_t)h * G + g) : -1;
+    if (((odd >> t) & 1) == 0) write_rows(a, dst, split, fq, r.o[t], r.lim[t] > 0.f ? -r.shift[t] : -INFINITY, r.l[t]);
+  }
+#pragma unroll 1
+  for (; odd; odd &= odd - 1) {
+    int token, g;
+    row_of(__builtin_ctz(odd), token, g);
+    const bool valid = token < q_len;
+    const size_t row = q_start + (valid ? token : 0), head = (size_t)h * G + g;
+    careful_tile<KV8>(a, table, h, sp, i0, i1, split, lane, a.q + row * a.q_stride + head * HD, valid ? first + token : -1,
+                      valid ? (int64_t)(row * a.n_q + head) : -1, is_inside);
   }
 }
 
@@ -868,7 +822,8 @@ __global__ __launch_bounds__(256) void window_join_kernel(WinArgs a) {
 
 int check_args(const WinArgs& a) {
   if (a.rows <= 0 || a.n_seqs <= 0 || a.n_seqs > 65535 || a.n_q <= 0 || a.n_kv <= 0 || a.n_q % a.n_kv != 0 || a.width <= 0 || a.pages <= 0 ||
-      a.q_stride < a.n_q * HD || a.q_stride % 8 != 0 || a.width > INT32_MAX / BLK - 2)
+      a.q_stride < a.n_q * HD || a.q_stride % 8 != 0 || a.width > INT32_MAX / BLK - 2 ||
+      (int64_t)a.pages * a.n_kv > INT32_MAX)
     return KLM_ERR_SHAPE;
   if (a.window < 1 || a.window > (1 << 30) || a.sinks < 0 || a.sinks > (1 << 30) || a.splits < 1 || a.splits > 256 || !(a.scale_log2 > 0.f))
     return KLM_ERR_ARG;
@@ -892,7 +847,7 @@ int launch_join(const WinArgs& a, hipStream_t s) {
 
 template <int QT, bool KV8>
 int launch_prefill(const WinArgs& a, hipStream_t s) {
-  constexpr int LDS = RING * STEP_BYTES + (KV8 ? 16384 : 0);
+  constexpr int LDS = (KV8 ? 6 : 4) * HALF;
   const int64_t tiles = ((int64_t)a.rows * a.G + 64 * QT - 1) / (64 * QT) + a.n_seqs;       // every sequence may end in a partial tile
   if (tiles > 65535 || (int64_t)a.rows * a.G > (1 << 30) || (a.splits > 1 && a.rows > 65535)) return KLM_ERR_SHAPE;
   if (klm_ensure_dyn_lds<window_prefill_kernel<QT, KV8>>(LDS) != KLM_OK) return KLM_ERR_HIP;
@@ -926,7 +881,7 @@ int klm_window_attn_prefill(const klm_window_args* c) {
   hipStream_t s = static_cast<hipStream_t>(c->stream);
   switch (c->q_tiles) {
     case 1: return c->kv_fp8 ? launch_prefill<1, true>(a, s) : launch_prefill<1, false>(a, s);
-    case 3: return c->kv_fp8 ? launch_prefill<3, true>(a, s) : launch_prefill<3, false>(a, s);
+    case 2: return c->kv_fp8 ? launch_prefill<2, true>(a, s) : launch_prefill<2, false>(a, s);
     default: return KLM_ERR_VARIANT;
   }
 }

@@ -706,18 +706,22 @@ def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int, s
     """(16-row tiles a wave, splits of the keys) of `paged_attn_prefill_window`: `reach` keys are the most that a query sees, `span`
     the most that a context has.
 
-    A block of 3 tiles a wave takes three times the rows for 2.1 times the time (1.7 and 0.8 us a 32-key step with the chip
-    full), one of a single tile leaves less idle where the last blocks run alone. MI355X, 32 query heads over 8 kv heads, one
-    whole prompt, whose first tiles see few keys: 2048 tokens (344 blocks of the large kind) 56 us with single tiles and 117
-    with three, 4096 (688) 183 and 234, 5000 (840) 268 and 287, 6144 (1032) 383 and 297. Chunks of a longer context, whose
-    tiles all see the same: 2048 queries behind 4000 keys (344) 156 and 181, the same with 64 heads (688) 293 and 264, 1200
-    with 64 heads (408) 180 and 138. Splits pay while single tiles leave CUs without a block: 16 queries over 4000 keys
-    11.8 us with 16 of them, 39 without; 500 queries 21.0 us without, 23.6 with 2."""
-    large = (rows * group // 192 + seqs) * n_kv
-    if large >= (380 if span > 1.5 * rows else 840):
-        return 3, 1
-    blocks = (-(-rows * group // 64) + seqs - 1) * n_kv
-    return 1, max(1, min(300 // blocks, (reach // 32 + 1) // 4, 16))
+    Two tiles a wave read the keys half as often but come in blocks of 128 rows, 768 of which are on the chip at once, against
+    1024 of 64: fewer blocks leave more idle at the end. MI355X, 32 query heads over 8 kv heads, with one and with two. One whole
+    prompt, whose first tiles see few keys: 2048 tokens (520 large blocks) 57 and 65 us, 4096 (1032) 159 and 148, 8192 (2056) 452
+    and 387. Chunks of a longer context, whose tiles all see the same: 1500 queries behind 4000 keys (376) 103 and 117, 2048 (520)
+    132 and 136, with an e4m3 cache 187 and 145, 4096 (1032) 278 and 268.
+
+    Splits pay while there are few blocks: a 32-key step takes 0.4 us, a split of a row costs 0.23 ns per query head for its part
+    to be written and joined. 16 queries over 4000 keys: 49 us in one, 11 in 16; 512 queries 58 in one, 45 in 4; 500 tokens that
+    are the whole prompt 14 in one, 19 in 2."""
+    large = (rows * group // 128 + seqs) * n_kv
+    if large >= (512 if span * seqs > 1.5 * rows else 900):
+        return 2, 1
+    blocks, steps = (-(-rows * group // 64) + seqs - 1) * n_kv, reach // 32 + 1
+    if steps < 8:
+        return 1, 1
+    return 1, max(1, min(int((1740 * steps / (rows * group * n_kv)) ** 0.5), 900 // blocks, steps // 2, 24))
 
 
 def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,

@@ -79,14 +79,14 @@ def test_window_refusals():
 
 def test_tiles_and_splits_of_a_prefill():
     pick = llm.pick_window_tiles
-    assert pick(8192, 1, 4, 8, 4100, 8192) == (3, 1) and pick(2048, 1, 4, 8, 2048, 2048) == (1, 1)
-    assert pick(1200, 1, 8, 8, 4096, 5200) == (3, 1)
-    assert pick(16, 1, 4, 8, 4096, 4016) == (1, 16) and pick(1, 1, 1, 1, 3, 16) == (1, 1)
+    assert pick(8192, 1, 4, 8, 4100, 8192) == (2, 1) and pick(2048, 1, 4, 8, 2048, 2048) == (1, 1)
+    assert pick(1200, 1, 8, 8, 4096, 5200) == (2, 1) and pick(500, 1, 4, 8, 500, 500) == (1, 1)
+    assert pick(16, 1, 4, 8, 4096, 4016) == (1, 20) and pick(1, 1, 1, 1, 3, 16) == (1, 1)
     for rows in (1, 7, 100, 3000):
         for seqs in (1, 5, 200):
             for group, n_kv in ((1, 1), (4, 8), (16, 2), (7, 3)):
                 tiles, splits = pick(rows, seqs, group, n_kv, 4096, 5000)
-                assert tiles in (1, 3) and 1 <= splits <= 16 and (splits == 1 or tiles == 1)
+                assert tiles in (1, 2) and 1 <= splits <= 24 and (splits == 1 or tiles == 1)
 
 
 # ---------------------------------------------------------------------------------------------------------------- pages
