@@ -1,7 +1,7 @@
 // Rules on logits and the greedy choice of a token. For a row x of logits, its history of prompt and output tokens and
 //   seen(v) = v is in the history, c(v) = how often v is in its output part
 //     x1 = seen(v) ? (x > 0 ? x / r : x * r) : x         repetition penalty r
-//     x2 = x1 - f * c(v)                                 frequency penalty f
+//     x2 = c(v) > 0 ? x1 - f * c(v) : x1                 frequency penalty f
 //     x3 = c(v) > 0 ? x2 - p : x2                        presence penalty p
 //     x4 = x3 + bias(v)                                  a token listed twice: the later entry counts
 //     y  = allowed(v) ? x4 : -inf                        a grammar's mask, one bit a token
@@ -71,9 +71,11 @@ __device__ __forceinline__ float apply_rules(float x, uint32_t cnt, float r, flo
   const float c = (float)(cnt & 0x7fffffffu);
   if (cnt != 0) {
     x = x > 0.f ? x / r : x * r;
-    const float fc = f * c;
-    x = x - fc;
-    if ((cnt & 0x7fffffffu) != 0) x = x - p;
+    if ((cnt & 0x7fffffffu) != 0) {
+      const float fc = f * c;
+      x = x - fc;
+      x = x - p;
+    }
   }
   return x;
 }

@@ -682,7 +682,8 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     if B == 0:
         return out
     window, sinks = min(window, _FAR), min(sinks, _FAR)
-    splits = num_splits or pick_window_splits(B * n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK))
+    splits = num_splits or min(pick_window_splits(B * n_kv * -(-n_q // n_kv // 16), min(window + sinks, width * BLOCK)),
+                               workspace.max_splits if workspace is not None else 256)
     part_o = part_ml = 0
     if splits > 1:
         if workspace is None:
@@ -841,7 +842,10 @@ def _few_pairs(pairs: list, src_nb: int, nb: int, same: bool) -> Optional[np.nda
 
 def _page_pairs(pairs, src_nb: int, nb: int, same: bool) -> np.ndarray:
     """The pairs as int32 [n, 2], checked (see copy_pages), without those of a page and itself."""
-    p = np.asarray(pairs)
+    try:
+        p = np.asarray(pairs)
+    except (TypeError, ValueError) as e:
+        raise KlmOpsError(f"copy_pages: pairs of two page numbers are wanted ({e})") from None
     if p.size == 0:
         return p.reshape(0, 2)
     if p.ndim != 2 or p.shape[1] != 2 or p.dtype.kind not in "iu":
@@ -957,7 +961,7 @@ def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, firs
     """Greedy choice under `rules` -> (token ids int64 [B], their processed logits fp32 [B]).
 
     For token v of a row: ``x = seen ? (x > 0 ? x / repetition : x * repetition) : x`` where `seen` is: v is in the history;
-    ``x -= frequency * c`` and, where c > 0, ``x -= presence``, c being how often v is in the history's output part;
+    where c > 0, c being how often v is in the history's output part, ``x -= frequency * c`` and ``x -= presence``;
     ``x += bias``; a token that the mask does not allow becomes -inf. Each step is rounded to fp32 by itself. The choice is the allowed token
     of the largest value, the lowest id among equals (NaN counts as largest, as in torch.argmax), -1 where none is allowed.
 

@@ -214,6 +214,7 @@ class Engine:
         self._store: Optional[RuleStore] = None           # made with the first request that has rules
         self._d_rows: Optional[torch.Tensor] = None       # decode row -> its set of rules
         self._step_lock = threading.RLock()               # a step, or a change of the cache between two steps
+        self._between = 0                                 # threads that wait for the time between two steps
         self._workspace = llm.DecodeWorkspace(B, self.lcfg.n_q, 64, dev) if self.on_gpu else None
 
     # ------------------------------------------------------------------ sizing
@@ -611,6 +612,15 @@ class Engine:
         needed. ValueError where the blocks would not hold what is in flight, or a request that waits, to its end."""
         if self.tp.world > 1:
             raise ValueError("resize_cache: the ranks of a tensor-parallel engine take the smallest count when they start")
+        with self._lock:
+            self._between += 1
+        try:
+            self._resize(num_blocks)
+        finally:
+            with self._lock:
+                self._between -= 1
+
+    def _resize(self, num_blocks: int) -> None:
         with self._step_lock, self._lock:
             live = self.prefilling + self.running
             held = sum(1 for r in live for b in r.blocks if b >= 0)
@@ -651,6 +661,8 @@ class Engine:
                     break
             elif self._stop.is_set():
                 break
+            while self._between:                          # the lock alone would go to this thread again and again
+                time.sleep(0.0002)
             try:
                 n = self.step()
                 if self.tp.world > 1 and n:

@@ -279,6 +279,18 @@ def test_captured_attention():
     _replays(lambda: [llm.paged_attn_prefill_window(q2, k2, v2, table2, info, SCALE, 16, 70, 4)], None, change2)
 
 
+def test_a_workspace_of_fewer_splits():
+    """The choice of splits keeps within the workspace; a number that is asked for and does not fit is refused."""
+    seqs = [900, 31, 0]
+    q, k, v, table = make("decode", seqs, 4, 1, 600, 4)
+    want, size = by_definition("decode", q, k, v, table, seqs, 4, 600, 4)
+    for most in (1, 2, 3):
+        ws = llm.DecodeWorkspace(4, 4, most, DEV)
+        _near(_decode(q, k, v, table, seqs, 4, 600, 4, workspace=ws), want, size)
+        with pytest.raises(KlmOpsError):
+            _decode(q, k, v, table, seqs, 4, 600, 4, workspace=ws, num_splits=most + 1)
+
+
 def test_two_streams_at_once():
     """Two calls in flight with the scratch of their own."""
     seqs = [4000] * 3

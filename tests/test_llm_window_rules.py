@@ -24,6 +24,15 @@ TINY = PRESETS["tiny"]
 WINDOW, SINKS = 37, 5
 
 
+@pytest.fixture(scope="module", autouse=True)
+def two_threads():
+    """The products here are small: more threads only add to the machine's load, which other tests look at."""
+    n = torch.get_num_threads()
+    torch.set_num_threads(min(n, 2))
+    yield
+    torch.set_num_threads(n)
+
+
 @pytest.fixture(scope="module")
 def model():
     torch.manual_seed(0)
@@ -247,6 +256,19 @@ def test_the_cache_changes_its_size_between_steps(which, request):
     assert not sizes
     for p, r in zip(prompts, reqs):
         assert r.error is None and r.out == dense_generate(m, p, 40, RULES[0])
+
+
+def test_the_size_changes_while_the_engine_thread_runs(model):
+    eng = engine(model, kv_blocks=64).start()
+    try:
+        reqs = [eng.submit(list(range(1, 30)), 60) for _ in range(4)]
+        for n in (40, 64, 50):
+            eng.resize_cache(n)                           # between two steps of the other thread, however busy it is
+        for r in reqs:
+            assert r.done.wait(60) and r.error is None and r.out == reqs[0].out
+        assert eng.alloc.total == 50 and reqs[0].out == dense_generate(model, list(range(1, 30)), 60)
+    finally:
+        eng.stop()
 
 
 def test_a_cache_too_small_for_what_is_in_flight_is_refused(model):

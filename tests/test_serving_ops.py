@@ -77,6 +77,19 @@ def test_window_refusals():
         llm.paged_attn_prefill_window(q, k, v, table, info, SCALE, 4, 0)
 
 
+def test_pairs_that_are_no_pairs_are_refused_alike():
+    """The check of short lists and that of all else take and refuse the same."""
+    k, v = torch.zeros(1, 8, 1, 16, 128), torch.zeros(1, 8, 1, 128, 16)
+    for bad in ([(1, 2, 3)], [(1, 2), (3,)], [1, 2], [(1.5, 2)], [("a", 1)], [(None, 1)], [(0, 8)], [(-2, 0)], [(8, 0)], [(2 ** 40, 0)], [(0, 1), (2, 1)],
+                [(0, 1), (1, 2)], [(0, 2 ** 70)]):
+        for pairs in (bad, tuple(bad), bad + [(4, i) for i in range(3, 3)]):
+            with pytest.raises(KlmOpsError):
+                llm.copy_pages(k, v, pairs)
+    for n in (1, 3):
+        for same in ([(1, 1)] * n if n == 1 else [(1, 1), (2, 2), (0, 3)], [[0, 5]], ((0, 5),), torch.tensor([[0, 5]])):
+            llm.copy_pages(k, v, same)
+
+
 def test_tiles_and_splits_of_a_prefill():
     pick = llm.pick_window_tiles
     assert pick(8192, 1, 4, 8, 4100, 8192) == (2, 1) and pick(2048, 1, 4, 8, 2048, 2048) == (1, 1)
