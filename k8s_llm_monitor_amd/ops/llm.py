@@ -28,11 +28,12 @@ rope_table = ref.rope_table
 
 _bound = False
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)       # of a process that has a tensor on a GPU
 
 
 def _stream(t: torch.Tensor) -> int:
     """The current stream of the tensor's device, as a number (2 us less than through a torch.cuda.Stream object)."""
-    return _raw_stream(t.device.index) if _raw_stream is not None else _stream_of(t)
+    return _raw_stream(t.get_device()) if _raw_stream is not None else _stream_of(t)
 
 
 def _lib():
@@ -610,20 +611,31 @@ def paged_attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
 
 # ------------------------------------------------------------------ sliding window and sinks
+_INF = float("inf")
 _FAR = 1 << 30          # a window or sinks beyond any context; keeps the kernels' 32-bit positions from running over
 _WINDOW_ARGS = struct.Struct("9P13if")          # klm_window_args
 
 
 def _call(fn, args: bytes, t: torch.Tensor) -> int:
     """A launcher on the device of `t`, whichever is current."""
-    if t.device.index == torch.cuda.current_device():
+    if t.get_device() == _current_device():
         return fn(args)
     with _on_device(t):
         return fn(args)
 
 
 def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q, window, sinks, out) -> None:
-    ks, dev = k_cache.shape, q.device
+    # the usual case in one expression; where it does not hold, what is wrong is named below
+    qs, ks, vs, at = q.shape, k_cache.shape, v_cache.shape, q.get_device()
+    if at >= 0 and len(qs) == 2 and len(ks) == len(vs) == 4 and ks[0] == vs[0] > 0 and ks[1] == vs[1] > 0 and \
+            ks[2] == BLOCK == vs[3] and ks[3] == HEAD_DIM == vs[2] and n_q > 0 and n_q % ks[1] == 0 and qs[1] >= n_q * HEAD_DIM and \
+            q.stride(1) == 1 and (qs[0] == 1 or q.stride(0) >= n_q * HEAD_DIM) and window > 0 and sinks >= 0 and 0.0 < scale < _INF and \
+            out is None and q.dtype is torch.bfloat16 and k_cache.dtype is v_cache.dtype and block_tables.dtype is torch.int32 and \
+            lens.dtype is torch.int32 and len(block_tables.shape) == 2 and block_tables.shape[1] > 0 and k_cache.is_contiguous() and \
+            v_cache.is_contiguous() and block_tables.is_contiguous() and lens.is_contiguous() and \
+            at == k_cache.get_device() == v_cache.get_device() == block_tables.get_device() == lens.get_device():
+        return
+    dev = q.device
     if len(ks) != 4 or len(v_cache.shape) != 4:
         raise KlmOpsError(f"{what}: cache shapes K {tuple(ks)} V {tuple(v_cache.shape)}")
     _check_caches(k_cache, v_cache, ks[1])
@@ -635,7 +647,7 @@ def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q
         raise KlmOpsError(f"{what}: block_tables {tuple(block_tables.shape)}")
     if window < 1 or sinks < 0:
         raise KlmOpsError(f"{what}: window {window} (at least 1: the token itself), sinks {sinks}")
-    if not 0.0 < scale < float("inf"):
+    if not 0.0 < scale < _INF:
         raise KlmOpsError(f"{what}: scale {scale}")
     if out is not None and (tuple(out.shape) != (q.shape[0], n_q * HEAD_DIM) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev):
         raise KlmOpsError(f"{what}: out {tuple(out.shape)} {out.dtype} {out.device}")
@@ -687,7 +699,7 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     part_o = part_ml = 0
     if splits > 1:
         if workspace is None:
-            scratch = torch.empty(B * n_q * splits * (HEAD_DIM + 2), dtype=torch.float32, device=q.device)
+            scratch = q.new_empty((B * n_q * splits * (HEAD_DIM + 2),), dtype=torch.float32)
             part_o = scratch.data_ptr()
             part_ml = part_o + B * n_q * splits * HEAD_DIM * 4
         else:
@@ -753,7 +765,7 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK), width * BLOCK)
     part_o = part_ml = 0
     if splits > 1:
-        scratch = torch.empty(T * n_q * splits * (HEAD_DIM + 2), dtype=torch.float32, device=q.device)
+        scratch = q.new_empty((T * n_q * splits * (HEAD_DIM + 2),), dtype=torch.float32)
         part_o = scratch.data_ptr()
         part_ml = part_o + T * n_q * splits * HEAD_DIM * 4
     rc = _call(_lib().klm_window_attn_prefill,
@@ -885,16 +897,17 @@ class LogitRules:
                  frequency: torch.Tensor, presence: torch.Tensor, bias_ids: Optional[torch.Tensor] = None,
                  bias_values: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                  mask_rows: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None):
-        self.__dict__.update(history=history, prompt_lens=prompt_lens, lens=lens, repetition=repetition, frequency=frequency,
-                             presence=presence, bias_ids=bias_ids, bias_values=bias_values, mask=mask, mask_rows=mask_rows, rows=rows)
-        i32, f32, R, device = torch.int32, torch.float32, lens.shape[0] if lens.dim() == 1 else -1, lens.device
+        d = self.__dict__
+        d["history"], d["prompt_lens"], d["lens"], d["repetition"], d["frequency"], d["presence"] = history, prompt_lens, lens, repetition, frequency, presence
+        d["bias_ids"], d["bias_values"], d["mask"], d["mask_rows"], d["rows"] = bias_ids, bias_values, mask, mask_rows, rows
+        i32, f32, R, at = torch.int32, torch.float32, lens.shape[0] if lens.dim() == 1 else -1, lens.get_device()
 
         def wants(name: str, t: torch.Tensor, dtype, *shape) -> None:
             """`shape`: a number, or None for any."""
             got = t.shape
             if t.dtype != dtype or len(got) != len(shape) or got[0] != (shape[0] if shape[0] is not None else got[0]) or \
-                    (len(shape) > 1 and got[1] != (shape[1] if shape[1] is not None else got[1])) or not t.is_contiguous() or t.device != device:
-                raise KlmOpsError(f"LogitRules: {name} must be contiguous {dtype} {list(shape)} on {device}, is {t.dtype} {list(got)} on {t.device}")
+                    (len(shape) > 1 and got[1] != (shape[1] if shape[1] is not None else got[1])) or not t.is_contiguous() or t.device != lens.device:
+                raise KlmOpsError(f"LogitRules: {name} must be contiguous {dtype} {list(shape)} on {lens.device}, is {t.dtype} {list(got)} on {t.device}")
 
         # the usual case in one expression; where it does not hold, the first that is wrong is named
         one = (R,)
@@ -902,7 +915,8 @@ class LogitRules:
                 repetition.dtype is f32 and frequency.dtype is f32 and presence.dtype is f32 and len(history.shape) == 2 and history.shape[0] == R and
                 repetition.shape == one == frequency.shape and presence.shape == one and history.is_contiguous() and
                 lens.is_contiguous() and prompt_lens.is_contiguous() and repetition.is_contiguous() and frequency.is_contiguous() and
-                presence.is_contiguous() and device == history.device == prompt_lens.device == repetition.device == frequency.device == presence.device):
+                presence.is_contiguous() and
+                at == history.get_device() == prompt_lens.get_device() == repetition.get_device() == frequency.get_device() == presence.get_device()):
             wants("lens", lens, i32, R)
             wants("prompt_lens", prompt_lens, i32, R)
             wants("history", history, i32, R, None)
@@ -943,13 +957,12 @@ class LogitRules:
 
     def _packed(self) -> Tuple[tuple, tuple]:
         """(addresses, sizes) as klm_logits_args has them."""
-        def at(t: Optional[torch.Tensor]) -> int:
-            return 0 if t is None else t.data_ptr()
-
-        n_masks, words = (0, 0) if self.mask is None else self.mask.shape
-        return ((at(self.rows), self.history.data_ptr(), self.prompt_lens.data_ptr(), self.lens.data_ptr(), self.repetition.data_ptr(),
-                 self.frequency.data_ptr(), self.presence.data_ptr(), at(self.bias_ids), at(self.bias_values), at(self.mask), at(self.mask_rows)),
-                (self.lens.shape[0], self.history.shape[1], 0 if self.bias_ids is None else self.bias_ids.shape[1], n_masks, words))
+        rows, ids, values, mask, mask_rows = self.rows, self.bias_ids, self.bias_values, self.mask, self.mask_rows
+        n_masks, words = (0, 0) if mask is None else mask.shape
+        return ((0 if rows is None else rows.data_ptr(), self.history.data_ptr(), self.prompt_lens.data_ptr(), self.lens.data_ptr(),
+                 self.repetition.data_ptr(), self.frequency.data_ptr(), self.presence.data_ptr(), 0 if ids is None else ids.data_ptr(),
+                 0 if values is None else values.data_ptr(), 0 if mask is None else mask.data_ptr(), 0 if mask_rows is None else mask_rows.data_ptr()),
+                (self.lens.shape[0], self.history.shape[1], 0 if ids is None else ids.shape[1], n_masks, words))
 
 
 _LOGITS_ARGS = struct.Struct("17Pq10i")          # klm_logits_args
