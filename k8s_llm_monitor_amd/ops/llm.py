@@ -844,10 +844,12 @@ def _few_pairs(pairs: list, src_nb: int, nb: int, same: bool) -> Optional[np.nda
     take both as long). None: something is out of order, `_page_pairs` sorts it out or says what it is."""
     try:
         to = {d: s for s, d in pairs}
-        if len(to) != len(pairs) or (same and not to.keys().isdisjoint(to.values())) or \
+        flat = [x for pair in pairs for x in pair]
+        # plain ints alone are equal when their numbers are: 0-d tensors, for one, hash by identity
+        if set(map(type, flat)) != {int} or len(to) != len(pairs) or (same and not to.keys().isdisjoint(to.values())) or \
                 not all(-1 <= s < src_nb and 0 <= d < nb for d, s in to.items()):
             return None
-        return np.frombuffer(array("i", [x for pair in pairs for x in pair]), dtype=np.int32).reshape(-1, 2)
+        return np.frombuffer(array("i", flat), dtype=np.int32).reshape(-1, 2)
     except (TypeError, ValueError, OverflowError):
         return None
 

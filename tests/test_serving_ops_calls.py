@@ -1,0 +1,34 @@
+"""Calls of the serving operators that their documentation allows or refuses and that tests/test_serving_ops.py does not make, on the
+CPU. The same operators on a GPU: tests/test_gpu_serving_ops.py, tests/test_gpu_serving_ops_calls.py."""
+import pytest
+import torch
+
+from k8s_llm_monitor_amd.ops import KlmOpsError, llm
+
+
+def _pages(blocks=8):
+    g = torch.Generator().manual_seed(0)
+    return torch.randn(2, blocks, 1, 16, 128, generator=g), torch.randn(2, blocks, 1, 128, 16, generator=g)
+
+
+# ---------------------------------------------------------------------------------------------------------------- pages
+@pytest.mark.parametrize("pairs", [[[0, 1], [2, 1]], [[0, 1], [1, 2]], [[-1, 1], [1, 2]], [[0, 8]], [[True, False]], [[0.0, 1.0]]])
+def test_pairs_are_looked_at_as_numbers_whatever_holds_them(pairs):
+    """A tensor of pairs, its rows in a list, its single numbers: a page written twice, or written and read, is refused in all forms."""
+    k, v = _pages()
+    k0 = k.clone()
+    t = torch.tensor(pairs)
+    for form in (pairs, tuple(map(tuple, pairs)), t, list(t), tuple(t), [tuple(row) for row in t], t.numpy(), list(t.numpy()), [tuple(row) for row in t.numpy()]):
+        with pytest.raises(KlmOpsError):
+            llm.copy_pages(k, v, form)
+    assert torch.equal(k, k0)
+
+
+def test_pairs_in_every_form_copy_the_same():
+    t = torch.tensor([[0, 5], [0, 6], [-1, 7]])
+    want = None
+    for form in (t.tolist(), t, list(t), [tuple(row) for row in t], t.numpy(), [tuple(row) for row in t.numpy()]):
+        k, v = _pages()
+        llm.copy_pages(k, v, form)
+        want = want or (k, v)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1]) and torch.equal(k[:, 5], k[:, 0]) and not v[:, 7].any()
