@@ -867,17 +867,17 @@ def _page_pairs(pairs, src_nb: int, nb: int, same: bool) -> np.ndarray:
     src, dst = p[:, 0], p[:, 1]
     if src.min() < -1 or src.max() >= src_nb or dst.min() < 0 or dst.max() >= nb:
         raise KlmOpsError(f"copy_pages: a pair outside the caches ({src_nb} and {nb} blocks; -1 clears)")
-    written = np.zeros(nb + 1, dtype=bool)                    # the place behind the last page stands for "nothing is read"
-    written[dst] = True
-    if np.count_nonzero(written) != len(p):
-        raise KlmOpsError("copy_pages: a page is written twice")
     if same:
         keep = src != dst
         if not keep.all():
             p = p[keep]
-            src = p[:, 0]
-        if written[src].any():                                # src -1 is that last place
-            raise KlmOpsError("copy_pages: a page is written by one pair and read by another")
+            src, dst = p[:, 0], p[:, 1]
+    written = np.zeros(nb + 1, dtype=bool)                    # the place behind the last page stands for "nothing is read"
+    written[dst] = True
+    if np.count_nonzero(written) != len(p):
+        raise KlmOpsError("copy_pages: a page is written twice")
+    if same and written[src].any():                           # src -1 is that last place
+        raise KlmOpsError("copy_pages: a page is written by one pair and read by another")
     return np.ascontiguousarray(p, dtype=np.int32)
 
 

@@ -32,3 +32,20 @@ def test_pairs_in_every_form_copy_the_same():
         llm.copy_pages(k, v, form)
         want = want or (k, v)
         assert torch.equal(k, want[0]) and torch.equal(v, want[1]) and torch.equal(k[:, 5], k[:, 0]) and not v[:, 7].any()
+
+
+def test_a_pair_of_a_page_and_itself_does_nothing():
+    """Neither counts as a write nor as a read of its page, but has to lie in the cache."""
+    for pairs, at in (([(3, 3), (3, 4)], [0, 1, 2, 3, 3, 5, 6, 7]), ([(3, 3), (0, 3)], [0, 1, 2, 0, 4, 5, 6, 7]), ([(3, 3), (3, 3)], list(range(8)))):
+        for form in (pairs, tuple(pairs), torch.tensor(pairs)):
+            k, v = _pages()
+            k0, v0 = k.clone(), v.clone()
+            llm.copy_pages(k, v, form)
+            assert torch.equal(k, k0[:, at]) and torch.equal(v, v0[:, at])
+    k, v = _pages()
+    for pairs in ([(8, 8)], [(-1, -1)], [(1, 1), (0, 1), (1, 2)], [(1, 1), (0, 1), (2, 1)]):
+        with pytest.raises(KlmOpsError):
+            llm.copy_pages(k, v, pairs)
+    k2, v2 = _pages()
+    with pytest.raises(KlmOpsError):                                     # another cache: the same number is another page
+        llm.copy_pages(k2, v2, [(3, 3), (0, 3)], k_src=k, v_src=v)
