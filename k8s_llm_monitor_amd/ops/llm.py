@@ -797,6 +797,15 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
 
 
+def _meets_rows(t: torch.Tensor, rows: torch.Tensor) -> bool:
+    """Does the contiguous tensor `t` share memory with a row of `rows` [B, V], which may be further apart than V?"""
+    if t.device != rows.device or not t.numel() or not rows.numel():
+        return False
+    at, end = t.data_ptr() - rows.data_ptr(), t.data_ptr() - rows.data_ptr() + t.numel() * t.element_size()
+    size, step = rows.shape[1] * rows.element_size(), max(1, rows.stride(0) * rows.element_size())
+    return max(0, (at - size) // step + 1) <= min(rows.shape[0] - 1, -(-end // step) - 1)        # first and last row that may
+
+
 def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs: Sequence[Tuple[int, int]],
                k_src: Optional[torch.Tensor] = None, v_src: Optional[torch.Tensor] = None) -> None:
     """Pages ``src -> dst`` of `pairs`, in every layer, K and V; ``src = -1`` clears the page to zeros.
@@ -993,7 +1002,7 @@ def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, firs
     if out is not None:
         if tuple(out.shape) != (B, V) or out.dtype != torch.float32 or not out.is_contiguous() or out.device != logits.device:
             raise KlmOpsError(f"{what}: out must be contiguous fp32 {[B, V]} on {logits.device}")
-        if _overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and logits.dtype == torch.float32 and logits.is_contiguous()):
+        if _meets_rows(out, logits) and not (out.data_ptr() == logits.data_ptr() and logits.dtype == torch.float32 and logits.is_contiguous()):
             raise KlmOpsError(f"{what}: out overlaps logits")
     if rules is not None:
         rules.check(B, first_token + V, logits.device)

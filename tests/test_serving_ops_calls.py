@@ -49,3 +49,25 @@ def test_a_pair_of_a_page_and_itself_does_nothing():
     k2, v2 = _pages()
     with pytest.raises(KlmOpsError):                                     # another cache: the same number is another page
         llm.copy_pages(k2, v2, [(3, 3), (0, 3)], k_src=k, v_src=v)
+
+
+# ------------------------------------------------------------------------------------------------------- rules on logits
+def test_out_may_not_share_memory_with_a_row_of_logits():
+    """Rows of logits far apart: `out` behind the first of them meets the last ones. Between them there is room."""
+    B, V = 4, 24
+    x = torch.randn(B, V, generator=torch.Generator().manual_seed(1))
+    flat = torch.zeros(2 * B * V)
+    for at in (0, 1, B * V - 7, B * V):
+        with pytest.raises(KlmOpsError):
+            llm.choose_tokens(flat.view(B, 2 * V)[:, :V], out=flat[at:at + B * V].view(B, V))
+    half = torch.zeros(3 * B * V, dtype=torch.bfloat16)
+    for at in (0, V, B * V // 2):
+        with pytest.raises(KlmOpsError):
+            llm.choose_tokens(half.view(B, 3 * V)[:, :V], out=half.view(torch.float32)[at:at + B * V].view(B, V))
+    room = torch.empty(8 * B * V)
+    for logits, at in ((room[:2 * B * V].view(B, 2 * V)[:, :V], 2 * B * V - V), (room[B * V:3 * B * V].view(B, 2 * V)[:, :V], 0),
+                       (room.view(B, 8 * V)[:, :V], V), (room.view(B, 8 * V)[:, :V], 17 * V)):
+        logits.copy_(x)
+        out = room[at:at + B * V].view(B, V)
+        ids, _ = llm.choose_tokens(logits, out=out)
+        assert torch.equal(out, x) and torch.equal(logits, x) and torch.equal(ids, x.argmax(-1))
