@@ -624,6 +624,15 @@ def _call(fn, args: bytes, t: torch.Tensor) -> int:
         return fn(args)
 
 
+def _meets_rows(t: torch.Tensor, rows: torch.Tensor, width: int) -> bool:
+    """Does the contiguous tensor `t` share memory with the first `width` places of a row of `rows`, which may be further apart?"""
+    if t.device != rows.device or not t.numel() or not rows.numel():
+        return False
+    at = t.data_ptr() - rows.data_ptr()
+    end, size, step = at + t.numel() * t.element_size(), width * rows.element_size(), max(1, rows.stride(0) * rows.element_size())
+    return max(0, (at - size) // step + 1) <= min(rows.shape[0] - 1, -(-end // step) - 1)        # first and last row that may
+
+
 def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q, window, sinks, out) -> None:
     # the usual case in one expression; where it does not hold, what is wrong is named below
     qs, ks, vs, at = q.shape, k_cache.shape, v_cache.shape, q.get_device()
@@ -651,6 +660,9 @@ def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q
         raise KlmOpsError(f"{what}: scale {scale}")
     if out is not None and (tuple(out.shape) != (q.shape[0], n_q * HEAD_DIM) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev):
         raise KlmOpsError(f"{what}: out {tuple(out.shape)} {out.dtype} {out.device}")
+    if out is not None and _meets_rows(out, q, n_q * HEAD_DIM) and \
+            (out.data_ptr() != q.data_ptr() or (q.shape[0] > 1 and q.stride(0) != n_q * HEAD_DIM)):
+        raise KlmOpsError(f"{what}: out shares a part of q's memory")
     if k_cache.device != dev or v_cache.device != dev or block_tables.device != dev or lens.device != dev:
         raise KlmOpsError(f"{what}: tensors on different devices")
     if q.is_cuda:
@@ -675,7 +687,8 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
 
     Pages between the sinks and the window are not looked at: their table entries may hold anything. An entry outside the
     cache (-1) is no page and its tokens are not seen, nor are tokens beyond the table. A sequence that sees nothing (length
-    0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `num_splits` 0: chosen from the shapes.
+    0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `out` may be `q` itself where that is contiguous, but
+    not share a part of it. `num_splits` 0: chosen from the shapes.
     `workspace`: the splits' scratch, for calls that must not take it from the allocator; calls that may run at the same time
     need one each."""
     what = "paged_attn_decode_window"
@@ -746,7 +759,7 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     No table of tiles: the kernel finds its work in `seq_info`, so nothing is computed on the host from the lengths and a
     captured call may be replayed with others. The sequences' rows must not overlap. A row of seq_info with q_len <= 0,
     ctx_len < q_len or queries that do not lie in q is no sequence. Rows of no sequence stay as they are in a given `out` and
-    are zero otherwise."""
+    are zero otherwise. `out` and `q`: as for the decode."""
     what = "paged_attn_prefill_window"
     _check_window(what, q, k_cache, v_cache, block_tables, seq_info, scale, n_q, window, sinks, out)
     S, width = block_tables.shape
@@ -795,15 +808,6 @@ def _page_shape(k: torch.Tensor, v: torch.Tensor) -> Tuple[int, int, int]:
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.device == b.device and a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and \
         b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
-
-
-def _meets_rows(t: torch.Tensor, rows: torch.Tensor) -> bool:
-    """Does the contiguous tensor `t` share memory with a row of `rows` [B, V], which may be further apart than V?"""
-    if t.device != rows.device or not t.numel() or not rows.numel():
-        return False
-    at, end = t.data_ptr() - rows.data_ptr(), t.data_ptr() - rows.data_ptr() + t.numel() * t.element_size()
-    size, step = rows.shape[1] * rows.element_size(), max(1, rows.stride(0) * rows.element_size())
-    return max(0, (at - size) // step + 1) <= min(rows.shape[0] - 1, -(-end // step) - 1)        # first and last row that may
 
 
 def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, pairs: Sequence[Tuple[int, int]],
@@ -1002,7 +1006,7 @@ def choose_tokens(logits: torch.Tensor, rules: Optional[LogitRules] = None, firs
     if out is not None:
         if tuple(out.shape) != (B, V) or out.dtype != torch.float32 or not out.is_contiguous() or out.device != logits.device:
             raise KlmOpsError(f"{what}: out must be contiguous fp32 {[B, V]} on {logits.device}")
-        if _meets_rows(out, logits) and not (out.data_ptr() == logits.data_ptr() and logits.dtype == torch.float32 and logits.is_contiguous()):
+        if _meets_rows(out, logits, V) and not (out.data_ptr() == logits.data_ptr() and logits.dtype == torch.float32 and logits.is_contiguous()):
             raise KlmOpsError(f"{what}: out overlaps logits")
     if rules is not None:
         rules.check(B, first_token + V, logits.device)

@@ -5,10 +5,39 @@ import torch
 
 from k8s_llm_monitor_amd.ops import KlmOpsError, llm
 
+from window_oracle import SCALE, make
+
 
 def _pages(blocks=8):
     g = torch.Generator().manual_seed(0)
     return torch.randn(2, blocks, 1, 16, 128, generator=g), torch.randn(2, blocks, 1, 128, 16, generator=g)
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("kind", ["decode", "prefill"])
+def test_attention_out_may_be_q_but_not_share_part_of_it(kind):
+    seqs = [20, 3, 40] if kind == "decode" else [(0, 2, 20), (2, 1, 3)]
+    q, k, v, table = make(kind, seqs, 4, 2, 8, 2, torch.float32)
+    q = q[:3].float()                                                     # contiguous [3, 512]
+    lens = torch.tensor(seqs, dtype=torch.int32)
+
+    def call(q, out=None):
+        f = llm.paged_attn_decode_window if kind == "decode" else llm.paged_attn_prefill_window
+        return f(q, k, v, table, lens, SCALE, 4, 8, 2, out=out)
+
+    want = call(q)
+    wide = torch.zeros(3, 1024)                                           # q as a part of fused rows
+    wide[:, :512] = q
+    for at in (0, 512, 1024, 1536):
+        with pytest.raises(KlmOpsError):
+            call(wide[:, :512], wide.view(-1)[at:at + 3 * 512].view(3, 512))
+    long = torch.zeros(5, 512)
+    long[:3] = q
+    with pytest.raises(KlmOpsError):
+        call(long[:3], long[1:4])
+    assert torch.equal(call(long[:3], long[3:5].repeat(2, 1)[:3]), want)
+    same = q.clone()
+    assert call(same, same) is same and torch.equal(same, want)
 
 
 # ---------------------------------------------------------------------------------------------------------------- pages
