@@ -511,14 +511,17 @@ class LlamaModel:
             vals, idx = out.float().max(dim=-1)
             idx = idx + tp.rank * vl
         else:
-            # -1: the rules allow no token of this rank's part; any token that another rank may choose goes before that
             idx, vals = llm.choose_tokens(out, rules, first_token=tp.rank * vl)
-            vals = torch.where(idx >= 0, vals.clamp(min=torch.finfo(torch.float32).min), -torch.inf)
         cand = torch.zeros((B + (B & 1), 2), dtype=torch.float32, device=out.device)
         cand[:B, 0] = vals
         cand[:B, 1] = idx.float()
         allc = tp.all_gather(cand)                                   # [world, B', 2]: the same bits on every rank
-        best = allc[:, :B, 0].argmax(dim=0)
+        best = allc[:, :B, 0]
+        if rules is not None:
+            # id -1: the rules allow no token of that rank's part; any allowed token goes before that, one of -inf too
+            there = allc[:, :B, 1] >= 0
+            best = (there & ((best == best.masked_fill(~there, -torch.inf).amax(dim=0)) | best.isnan())).float()
+        best = best.argmax(dim=0)
         return allc[:, :B, 1].gather(0, best[None])[0].long()
 
     def prefill(self, tokens, positions, slots, cache: KVCache, meta: PrefillMeta, logits: bool = False,

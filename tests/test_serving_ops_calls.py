@@ -1,8 +1,11 @@
 """Calls of the serving operators that their documentation allows or refuses and that tests/test_serving_ops.py does not make, on the
 CPU. The same operators on a GPU: tests/test_gpu_serving_ops.py, tests/test_gpu_serving_ops_calls.py."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
+from k8s_llm_monitor_amd.models.llama import LlamaModel
 from k8s_llm_monitor_amd.ops import KlmOpsError, llm
 
 from window_oracle import SCALE, make
@@ -100,3 +103,33 @@ def test_out_may_not_share_memory_with_a_row_of_logits():
         out = room[at:at + B * V].view(B, V)
         ids, _ = llm.choose_tokens(logits, out=out)
         assert torch.equal(out, x) and torch.equal(logits, x) and torch.equal(ids, x.argmax(-1))
+
+
+class _Ranks:
+    """Two ranks' `all_gather`, one after the other: the first round collects, the second answers with what both gave."""
+
+    def __init__(self):
+        self.world, self.rank, self.given = 2, 0, {}
+
+    def all_gather(self, x):
+        self.given[self.rank] = x.clone()
+        return torch.stack([self.given.get(r, x) for r in range(2)])
+
+
+@pytest.mark.parametrize("low", [-float("inf"), torch.finfo(torch.float32).min, -3.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("high", [-float("inf"), torch.finfo(torch.float32).min, 5.0, float("nan")])
+@pytest.mark.parametrize("allowed", [0b11, 0b10, 0b01, 0b00])
+def test_two_ranks_choose_what_one_would(low, high, allowed):
+    """Values at the ends of fp32 too: rank 0's tokens are all `low`, rank 1's all `high`; `allowed`: whose tokens the rules allow."""
+    V, z, one = 32, torch.zeros(3, dtype=torch.int32), torch.ones(3)
+    whole = torch.cat([torch.full((3, V), low), torch.full((3, V), high)], 1)
+    mask = torch.tensor([[-(allowed & 1), -(allowed >> 1)]] * 3, dtype=torch.int32)
+    rules = llm.LogitRules(torch.zeros(3, 1, dtype=torch.int32), z, z, one, one * 0, one * 0, mask=mask)
+    want = llm.choose_tokens(whole, rules)[0]
+    tp = _Ranks()
+    model = SimpleNamespace(tp=tp)
+    for _ in range(2):
+        got = []
+        for tp.rank in range(2):
+            got.append(LlamaModel._sample(model, whole[:, tp.rank * V:(tp.rank + 1) * V].contiguous(), False, rules))
+    assert got[0].tolist() == got[1].tolist() == want.tolist()
