@@ -235,7 +235,7 @@ class Engine:
     def submit(self, prompt: Sequence[int], max_tokens: int = 16, rules: Optional[TokenRules] = None) -> Request:
         """`rules`: on the choice of this request's tokens (ValueError if they do not fit the vocabulary)."""
         if rules is not None:
-            rules.check(self.mcfg.vocab)
+            rules = rules.check(self.mcfg.vocab)
         now = self.clock()
         with self._lock:
             r = Request(self._next_id, [int(t) % self.mcfg.vocab for t in prompt], int(max_tokens), now, rules=rules)

@@ -6,6 +6,8 @@ No reference counterpart (vLLM is a README bullet in the reference, README.md:73
 from __future__ import annotations
 
 import math
+import numbers
+import operator
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -27,15 +29,31 @@ class TokenRules:
     allowed: Optional[Tuple[int, ...]] = None
 
     def check(self, vocab: int) -> "TokenRules":
-        """ValueError unless every number is finite and in range for a vocabulary of `vocab` tokens."""
-        numbers = (self.repetition, self.frequency, self.presence, *self.bias.values())
-        if not all(math.isfinite(x) and abs(x) <= 1e30 for x in numbers) or not 1e-30 <= self.repetition:
+        """These rules in plain ints and floats; ValueError unless every number is one, finite and in range for a vocabulary of
+        `vocab` tokens, and every token a whole number below that."""
+        def number(x) -> float:
+            if isinstance(x, bool) or not isinstance(x, numbers.Real):
+                raise ValueError(f"rules: {x!r} is no number")
+            return float(x)
+
+        def token(t) -> int:
+            if isinstance(t, bool):
+                raise ValueError(f"rules: {t!r} is no token")
+            return operator.index(t)
+
+        try:
+            penalties = number(self.repetition), number(self.frequency), number(self.presence)
+            bias = {token(t): number(x) for t, x in self.bias.items()}
+            allowed = None if self.allowed is None else tuple(token(t) for t in self.allowed)
+        except (TypeError, OverflowError, AttributeError) as e:
+            raise ValueError(f"rules: {e}") from None
+        if not all(math.isfinite(x) and abs(x) <= 1e30 for x in (*penalties, *bias.values())) or not 1e-30 <= penalties[0]:
             raise ValueError("rules: penalties and biases must be finite numbers, the repetition penalty above 0")
-        if len(self.bias) > MAX_BIASES or not all(0 <= t < vocab for t in self.bias):
+        if len(bias) > MAX_BIASES or not all(0 <= t < vocab for t in bias):
             raise ValueError(f"rules: at most {MAX_BIASES} biases, of tokens below {vocab}")
-        if self.allowed is not None and (not self.allowed or not all(0 <= t < vocab for t in self.allowed)):
+        if allowed is not None and (not allowed or not all(0 <= t < vocab for t in allowed)):
             raise ValueError(f"rules: allowed tokens must be a list of one token below {vocab} at least")
-        return self
+        return TokenRules(*penalties, bias, allowed)
 
     @staticmethod
     def from_request(req: dict, vocab: int) -> Optional["TokenRules"]:
