@@ -70,7 +70,8 @@ class TokenRules:
                 raise ValueError(f"{key} must be a number")
             return float(x)
 
-        bias, allowed = req.get("logit_bias") or {}, req.get("allowed_token_ids")
+        bias, allowed = req.get("logit_bias"), req.get("allowed_token_ids")
+        bias = {} if bias is None else bias
         if not isinstance(bias, dict) or any(isinstance(x, bool) or not isinstance(x, (int, float)) for x in bias.values()):
             raise ValueError("logit_bias must map token ids to numbers")
         if allowed is not None and not (isinstance(allowed, list) and all(isinstance(t, int) and not isinstance(t, bool) for t in allowed)):

@@ -68,3 +68,14 @@ def test_what_was_submitted_is_what_holds(model):
     b = eng.submit(PROMPT, 6, TokenRules(bias={7: 2.0}))
     drain(eng)
     assert a.error is None and beside.error is None and a.out == b.out and len(beside.out) == 6
+
+
+@pytest.mark.parametrize("bias", [[], 0, False, "", [1], 1.5])
+def test_a_request_whose_biases_are_no_map_is_refused(bias):
+    with pytest.raises(ValueError):
+        TokenRules.from_request({"logit_bias": bias}, 512)
+
+
+def test_a_request_without_rules_has_none():
+    assert TokenRules.from_request({"prompt": [1], "logit_bias": None, "allowed_token_ids": None}, 512) is None
+    assert TokenRules.from_request({"logit_bias": {}}, 512) == TokenRules()
