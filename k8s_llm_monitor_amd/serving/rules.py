@@ -103,6 +103,14 @@ class RuleStore:
 
     def take(self, rules: TokenRules, prompt_len: int) -> int:
         i = self._free.pop()
+        try:
+            self._fill(i, rules, prompt_len)
+        except BaseException:
+            self._free.append(i)
+            raise
+        return i
+
+    def _fill(self, i: int, rules: TokenRules, prompt_len: int) -> None:
         ids = np.full(MAX_BIASES, -1, dtype=np.int32)
         values = np.zeros(MAX_BIASES, dtype=np.float32)
         ids[:len(rules.bias)] = list(rules.bias)
@@ -117,7 +125,6 @@ class RuleStore:
             self.mask[i].copy_(torch.from_numpy(np.packbits(bits, bitorder="little").view("<i4").astype(np.int32)))
         self.mask_rows[i] = i if rules.allowed is not None else -1
         self._known[i] = 0
-        return i
 
     def give_back(self, i: int) -> None:
         self._free.append(i)

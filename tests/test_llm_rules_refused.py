@@ -79,3 +79,27 @@ def test_a_request_whose_biases_are_no_map_is_refused(bias):
 def test_a_request_without_rules_has_none():
     assert TokenRules.from_request({"prompt": [1], "logit_bias": None, "allowed_token_ids": None}, 512) is None
     assert TokenRules.from_request({"logit_bias": {}}, 512) == TokenRules()
+
+
+def test_a_set_of_rules_comes_back_from_a_step_that_failed_to_fill_it(model, monkeypatch):
+    eng = engine(model)
+    one = eng.submit(PROMPT, 3, TokenRules(repetition=1.5))
+    drain(eng)
+    store, rules = eng._store, TokenRules(repetition=1.5, allowed=(1, 2, 3))
+    for what in ("history", "bias_ids", "bias_values", "penalties", "prompt_lens", "mask", "mask_rows"):
+        tensor = getattr(store, what)
+        if what != "history":                            # (`follow` writes it, after the set has been taken)
+            monkeypatch.setattr(store, what, None)
+            with pytest.raises((TypeError, AttributeError)):
+                store.take(rules, 3)
+            assert sorted(store._free) == [0, 1], what
+        monkeypatch.setattr(store, what, None)
+        r = eng.submit(PROMPT, 3, rules)
+        with pytest.raises((TypeError, AttributeError)):
+            eng.step()
+        eng._fail_all("for the test")
+        assert r.error and sorted(store._free) == [0, 1], what
+        monkeypatch.setattr(store, what, tensor)
+    again = eng.submit(PROMPT, 3, TokenRules(repetition=1.5))
+    drain(eng)
+    assert again.error is None and again.out == one.out
