@@ -390,8 +390,8 @@ class Engine:
         if all(r.rules is None for r in reqs):
             return None
         if self._store is None:
-            self._store = RuleStore(self.cfg.max_num_seqs, self.max_len, self.mcfg.vocab, self.device)
             self._d_rows = torch.full((self.cfg.max_num_seqs,), -1, dtype=torch.int32, device=self.device)
+            self._store = RuleStore(self.cfg.max_num_seqs, self.max_len, self.mcfg.vocab, self.device)
         for r in reqs:
             if r.rules is not None and r.rule_set < 0:
                 r.rule_set = self._store.take(r.rules, len(r.prompt))

@@ -103,3 +103,21 @@ def test_a_set_of_rules_comes_back_from_a_step_that_failed_to_fill_it(model, mon
     again = eng.submit(PROMPT, 3, TokenRules(repetition=1.5))
     drain(eng)
     assert again.error is None and again.out == one.out
+
+
+def test_an_engine_whose_first_step_with_rules_failed_serves_the_next(model, monkeypatch):
+    eng = engine(model)
+    full = torch.full
+
+    def no_memory(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    eng.submit(PROMPT, 3, TokenRules(repetition=1.5))
+    monkeypatch.setattr(torch, "full", no_memory)
+    with pytest.raises(RuntimeError):
+        eng.step()
+    monkeypatch.setattr(torch, "full", full)
+    eng._fail_all("for the test")
+    r = eng.submit(PROMPT, 3, TokenRules(repetition=1.5))
+    drain(eng)
+    assert r.error is None and len(r.out) == 3
