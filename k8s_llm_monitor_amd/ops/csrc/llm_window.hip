@@ -294,7 +294,7 @@ __device__ __forceinline__ int k_key(int tok) { return (tok & 3) | (((tok >> 3) 
 // behind the first, in memory as in LDS.
 // Written in assembly because the compiler takes the builtin for an access that may hit LDS at any time, and then waits for all
 // outstanding LDS reads at each of them (and for the DMA before them); what has landed is said by the kernel's own waits. No
-// register is written but m0, which nothing else here uses. s_nop 4: a scalar base that a vector instruction wrote may be
+// register is written but m0. s_nop 4: a scalar base that a vector instruction wrote may be
 // read by a memory instruction five states later; s_nop 0: m0 before its use.
 __device__ __forceinline__ void dma_step(const WinArgs& a, int at, uint32_t st, int w, unsigned ko, unsigned vo) {
   const size_t base = (size_t)(at < 0 ? 0 : at) * (BLK_ELEMS * 2);
@@ -311,7 +311,7 @@ __device__ __forceinline__ void dma_step(const WinArgs& a, int at, uint32_t st, 
       "global_load_lds_dwordx4 %1, %3 offset:1024"
       :
       : "v"(ko), "v"(vo), "s"(k), "s"(v), "s"(st + w * 2048), "s"(st + 2 * HALF + w * 2048)
-      : "memory");
+      : "memory", "m0");
 }
 
 // The same of an e4m3 cache: a wave's 2 KiB of raw bytes go to a corner of its own, `raw`, from where it turns them into the bf16
@@ -329,7 +329,7 @@ __device__ __forceinline__ void dma_step8(const WinArgs& a, int at, uint32_t raw
       "global_load_lds_dwordx4 %0, %2"
       :
       : "v"(off), "s"(k), "s"(v), "s"(raw), "s"(raw + 1024)
-      : "memory");
+      : "memory", "m0");
 }
 __device__ __forceinline__ void widen_step8(char* st, const char* raw, int w, int lane) {
   const uint4 k = *reinterpret_cast<const uint4*>(raw + lane * 16), v = *reinterpret_cast<const uint4*>(raw + 1024 + lane * 16);
