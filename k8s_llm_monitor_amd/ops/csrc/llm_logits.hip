@@ -45,6 +45,8 @@ struct LogitArgs {
 // A block takes SLICE columns, a chunk of 8 a thread. Columns are counted from the 16-byte boundary at or before the
 // row's start, so that every chunk but a row's first and last is whole aligned loads whatever the row stride is.
 constexpr int THREADS = 512, SLICE = THREADS * 8;
+// Blocks on the chip at once: 3 per CU, 6 waves a SIMD of up to 80 registers (the four kernels take 70 to 76; LDS would hold 5).
+constexpr int RESIDENT = 3 * 256;
 
 // larger number = larger value; -0 and +0 are equal, a NaN is above everything; 0 is left for "no token"
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -119,7 +121,7 @@ __device__ __forceinline__ void load_bits(const uint32_t* mask, int words, int64
 }
 
 template <bool F32, bool BIAS>
-__global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs a, int slices, int per, int wide_out) {
+__global__ __launch_bounds__(THREADS, 6) void logits_kernel(LogitArgs a, int slices, int per, int wide_out) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   uint32_t* cnt = lds;                 // [SLICE] bit 31: in the prompt; below: times in the output
   uint32_t* last = lds + SLICE;        // [SLICE] 1 + the last bias entry of the token
@@ -300,12 +302,15 @@ __global__ __launch_bounds__(64) void choose_kernel(LogitArgs a, int parts) {
 }
 
 int slices_of(int V) { return (int)(((int64_t)V + 7 + SLICE - 1) / SLICE); }     // a row may start up to 7 places into its first slice
-// Slices that one block walks: as few as let all blocks be on the chip at once (4 per CU). A block's chain of dependent loads
-// (the row's lengths, its history, the mask) is longer than the work of a slice: 96 x 128256 in rounds of one slice 18.9 us.
+// Slices that one block walks: as few as let all blocks be on the chip at once, 8 at most. A block's chain of dependent loads (the
+// row's lengths, its history, the mask) is longer than the work of a slice, and a second round runs it again: 256 x 64128 fp32, 8
+// biases, processed logits written, 28.2 us with 6 slices a block (768 blocks), 31.6 with 4 (1024) and 37.9 with 1 (4096); 128 x
+// 128256, 2000 tokens of history, 22.5 with 6 (768), 25.7 with 4 (1024), 32.1 with 1 (4096). More slices than it takes leave CUs
+// idle: 96 x 128256 20.7 with 4 (768), 25.8 with 6 (576).
 int slices_per_block(int B, int V) {
   const int slices = slices_of(V);
   int per = 1;
-  while (per < 8 && (int64_t)((slices + per - 1) / per) * B > 1024) ++per;
+  while (per < 8 && (int64_t)((slices + per - 1) / per) * B > RESIDENT) ++per;
   return per;
 }
 

@@ -133,3 +133,13 @@ def test_two_ranks_choose_what_one_would(low, high, allowed):
         for tp.rank in range(2):
             got.append(LlamaModel._sample(model, whole[:, tp.rank * V:(tp.rank + 1) * V].contiguous(), False, rules))
     assert got[0].tolist() == got[1].tolist() == want.tolist()
+
+
+def test_blocks_of_a_choice_are_on_the_chip_at_once():
+    """3 blocks a CU of 256 CUs, where 8 slices a block are enough for that."""
+    for B in (1, 2, 7, 33, 64, 96, 128, 200, 256, 700):
+        for V in (1, 4090, 32000, 50001, 64128, 128256):
+            parts, slices = llm._lib().klm_logits_parts(B, V), -(-(V + 7) // 4096)
+            per = -(-slices // parts)
+            assert parts * B <= 768 or parts == -(-slices // 8), (B, V)
+            assert per == 1 or -(-slices // (per - 1)) * B > 768, (B, V)       # and no fewer blocks than that takes
