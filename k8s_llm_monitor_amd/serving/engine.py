@@ -638,6 +638,9 @@ class Engine:
             self._graphs.clear()
             self._rule_graphs.clear()
             self.cache, self.alloc = cache, alloc
+            del old
+            if self.on_gpu:
+                torch.cuda.empty_cache()                  # the old cache's memory to the device, not only to this process's allocator
             self.metrics.set_queue(len(self.running), len(self.waiting), alloc.usage)
 
     # ------------------------------------------------------------------ background loop

@@ -1,10 +1,14 @@
 """Calls of the serving operators that tests/test_gpu_serving_ops.py does not make, on the GPU: see tests/test_serving_ops_calls.py."""
+from dataclasses import replace
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
+from k8s_llm_monitor_amd.models.llama import PRESETS, LlamaModel  # noqa: E402
 from k8s_llm_monitor_amd.ops import KlmOpsError, llm  # noqa: E402
+from k8s_llm_monitor_amd.serving import Engine, EngineConfig, TokenRules  # noqa: E402
 
 from window_oracle import SCALE, make  # noqa: E402
 
@@ -64,3 +68,19 @@ def test_out_beside_and_between_rows_of_logits():
     logits.copy_(x)
     ids, best = llm.choose_tokens(logits, out=out)
     assert torch.equal(out, x) and torch.equal(logits, x) and torch.equal(ids, x.argmax(-1)) and torch.equal(best, x.amax(-1))
+
+
+# --------------------------------------------------------------------------------------------------------------- engine
+def test_a_smaller_cache_gives_its_memory_back():
+    """To the device, not only to the process's allocator: another process may have it."""
+    model = LlamaModel(replace(PRESETS["small"], window=50, sinks=4), "cuda", seed=3)
+    eng = Engine(EngineConfig(model="small", max_num_seqs=4, max_model_len=256, kv_blocks=16384), model=model)
+    reqs = [eng.submit(list(range(1, 30 + i)), 30, TokenRules(repetition=1.5) if i else None) for i in range(3)]
+    for _ in range(8):
+        eng.step()
+    size, before = eng.cache.nbytes, torch.cuda.memory_reserved()
+    eng.resize_cache(100)
+    assert size > 1 << 30 and eng.cache.nbytes < size // 100 and before - torch.cuda.memory_reserved() > size * 9 // 10
+    while not eng.idle():
+        eng.step()
+    assert all(r.error is None and len(r.out) == 30 for r in reqs)
