@@ -686,11 +686,10 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     ``j > position - window or j < sinks``.
 
     Pages between the sinks and the window are not looked at: their table entries may hold anything. An entry outside the
-    cache (-1) is no page and its tokens are not seen, nor are tokens beyond the table. A sequence that sees nothing (length
-    0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `out` may be `q` itself where that is contiguous, but
-    not share a part of it. `num_splits` 0: chosen from the shapes.
-    `workspace`: the splits' scratch, for calls that must not take it from the allocator; calls that may run at the same time
-    need one each."""
+    cache (-1) is no page and its tokens are not seen, nor are tokens beyond the table. A sequence that sees nothing
+    (length 0) gives zeros. Any number of query heads per kv head; bf16 and e4m3 caches. `out` may be `q` itself where
+    that is contiguous, but not share a part of it. `num_splits` 0: chosen from the shapes. `workspace`: the splits'
+    scratch, for calls that must not take it from the allocator; calls that may run at the same time need one each."""
     what = "paged_attn_decode_window"
     _check_window(what, q, k_cache, v_cache, block_tables, ctx_lens, scale, n_q, window, sinks, out)
     B, width = block_tables.shape
@@ -728,26 +727,29 @@ def paged_attn_decode_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     return out
 
 
-def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int, span: int) -> Tuple[int, int]:
+def pick_window_tiles(rows: int, seqs: int, group: int, n_kv: int, reach: int, span: int, kv8: bool = False) -> Tuple[int, int]:
     """(16-row tiles a wave, splits of the keys) of `paged_attn_prefill_window`: `reach` keys are the most that a query sees, `span`
-    the most that a context has.
+    the most that a context has. `kv8`: an e4m3 cache.
 
-    Two tiles a wave read the keys half as often but come in blocks of 128 rows, 768 of which are on the chip at once, against
-    1024 of 64: fewer blocks leave more idle at the end. MI355X, 32 query heads over 8 kv heads, with one and with two. One whole
-    prompt, whose first tiles see few keys: 2048 tokens (520 large blocks) 57 and 65 us, 4096 (1032) 159 and 148, 8192 (2056) 452
-    and 387. Chunks of a longer context, whose tiles all see the same: 1500 queries behind 4000 keys (376) 103 and 117, 2048 (520)
-    132 and 136, with an e4m3 cache 187 and 145, 4096 (1032) 278 and 268.
+    Two tiles a wave read the keys half as often but come in blocks of 128 rows, 768 of which are on the chip at once,
+    against 1024 of 64 (e4m3: 768 too, a block takes 48 KiB of LDS): fewer blocks leave more idle at the end. MI355X, 32
+    query heads over 8 kv heads, with one and with two. One whole prompt, whose first tiles see few keys: 2048 tokens (520
+    large blocks) 57 and 65 us, 4096 (1032) 159 and 148, 8192 (2056) 452 and 387. Chunks of a longer context, whose tiles
+    all see the same: 1500 queries behind 4000 keys (376) 103 and 117, 2048 (520) 132 and 136, with an e4m3 cache 187 and
+    145, 4096 (1032) 278 and 268.
 
-    Splits pay while there are few blocks: a 32-key step takes 0.4 us, a split of a row costs 0.23 ns per query head for its part
-    to be written and joined. 16 queries over 4000 keys: 49 us in one, 11 in 16; 512 queries 58 in one, 45 in 4; 500 tokens that
-    are the whole prompt 14 in one, 19 in 2."""
+    Splits pay while there are few blocks: a 32-key step takes 0.4 us, a split of a row costs 0.23 ns per query head for
+    its part to be written and joined. 16 queries over 4000 keys: 49 us in one, 11 in 16; 512 queries 58 in one, 45 in 4;
+    500 tokens that are the whole prompt 14 in one, 19 in 2. No more blocks than are on the chip at once; 800 queries over
+    4000 keys (400 blocks) 68 us in two, 69 in one, e4m3 94 and 85; 520 (264 blocks) 50 us in three, 53 in two, e4m3 65
+    and 62."""
     large = (rows * group // 128 + seqs) * n_kv
     if large >= (512 if span * seqs > 1.5 * rows else 900):
         return 2, 1
     blocks, steps = (-(-rows * group // 64) + seqs - 1) * n_kv, reach // 32 + 1
     if steps < 8:
         return 1, 1
-    return 1, max(1, min(int((1740 * steps / (rows * group * n_kv)) ** 0.5), 900 // blocks, steps // 2, 24))
+    return 1, max(1, min(int((1740 * steps / (rows * group * n_kv)) ** 0.5), (768 if kv8 else 900) // blocks, steps // 2, 24))
 
 
 def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -775,7 +777,8 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if zero_rest:
         out = q.new_empty((T, n_q * HEAD_DIM))
     window, sinks = min(window, _FAR), min(sinks, _FAR)
-    q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK), width * BLOCK)
+    kv8 = _kv8(k_cache)
+    q_tiles, splits = pick_window_tiles(T, S, n_q // n_kv, n_kv, min(window + sinks, width * BLOCK), width * BLOCK, kv8)
     part_o = part_ml = 0
     if splits > 1:
         scratch = q.new_empty((T * n_q * splits * (HEAD_DIM + 2),), dtype=torch.float32)
@@ -784,7 +787,7 @@ def paged_attn_prefill_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     rc = _call(_lib().klm_window_attn_prefill,
                _WINDOW_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), seq_info.data_ptr(),
                                  out.data_ptr(), part_o, part_ml, _stream(q), S, T, q.stride(0) if T > 1 else n_q * HEAD_DIM, n_q, n_kv, width, nb,
-                                 window, sinks, splits, _kv8(k_cache), q_tiles, zero_rest, scale), q)
+                                 window, sinks, splits, kv8, q_tiles, zero_rest, scale), q)
     if rc:
         _check(rc, f"klm_window_attn_prefill(T={T},S={S},window={window},sinks={sinks})")
     return out

@@ -43,6 +43,20 @@ def test_attention_out_may_be_q_but_not_share_part_of_it(kind):
     assert call(same, same) is same and torch.equal(same, want)
 
 
+def test_splits_of_a_prefill_stay_on_the_chip():
+    """1024 blocks of a bf16 cache, 768 of an e4m3 one: more would run as a whole round and a rest."""
+    pick = llm.pick_window_tiles
+    assert pick(800, 1, 4, 8, 4100, 4816, False) == (1, 2) and pick(800, 1, 4, 8, 4100, 4816, True) == (1, 1)
+    assert pick(520, 1, 4, 8, 4100, 4528, False) == (1, 3) and pick(520, 1, 4, 8, 4100, 4528, True) == (1, 2)
+    assert pick(16, 1, 4, 8, 4096, 4016) == pick(16, 1, 4, 8, 4096, 4016, True) == (1, 20)
+    for rows in (1, 60, 200, 390, 700, 900, 3000):
+        for seqs in (1, 5, 40):
+            for group, n_kv in ((1, 1), (4, 8), (16, 2), (7, 3), (8, 8)):
+                for kv8, most in ((False, 1024), (True, 768)):
+                    tiles, splits = pick(rows, seqs, group, n_kv, 4096, 5000, kv8)
+                    assert splits == 1 or (tiles == 1 and splits * (-(-rows * group // 64) + seqs - 1) * n_kv <= most)
+
+
 # ---------------------------------------------------------------------------------------------------------------- pages
 @pytest.mark.parametrize("pairs", [[[0, 1], [2, 1]], [[0, 1], [1, 2]], [[-1, 1], [1, 2]], [[0, 8]], [[True, False]], [[0.0, 1.0]]])
 def test_pairs_are_looked_at_as_numbers_whatever_holds_them(pairs):
