@@ -7,6 +7,12 @@
 // sinks and the window are never looked at, so the engine gives them back while the sequence runs. A row that sees nothing
 // gives 0. A masked key contributes nothing whatever its bytes are (stale slots, NaN, infinities).
 //
+// Roundings: scores, maxima, sums and the output's sums are fp32. A weight is rounded to bf16 before it meets V, because the matrix
+// instruction takes bf16: off by at most 2^-8 of itself. Its sum is taken unrounded, so that the two do not cancel: the result is
+// within 2^-8 sum p |v|, and 2^-8 of itself from its own rounding, of the formula. Un-normalised sums bound V: weights are at most 1
+// in the decode, at most 256 in the prefill, so that |V| times the keys, times 256 in the prefill, has to stay within fp32 (over a
+// million keys V up to 1e30 does).
+//
 // No reference counterpart (vLLM is a README bullet in the reference, README.md:73).
 #include <type_traits>
 
@@ -276,11 +282,12 @@ __global__ __launch_bounds__(256, 2) void window_decode_kernel(WinArgs a, int he
 // one is worked on the next is brought in, a bf16 cache by LDS-DMA (4 KiB a wave, no registers), an e4m3 cache by LDS-DMA as it
 // is and turned into bf16 once per block.
 // What bounds it: a step of two tiles is 32 matrix instructions (512 clocks) and 80 vector ones, 16 of them exp2 (400); with three
-// waves a SIMD they fill 55 and 45 % of the time, the rest waits on LDS and the barrier. Two tiles, because they and their state
-// fit 168 registers, three blocks a CU; three tiles at two blocks a CU, with the scores of a step computed under the weights of
-// the one before, took 391 us where this takes 384 (8192 tokens, 32 heads over 8, window 4096: 1075 TFLOP/s) and 293 where this
-// takes 260 (e4m3, chunks of a long context). One tile for fewer rows: 128 registers, four blocks a CU. A third step in LDS, wave
-// priorities and sums by matrix instructions gave nothing.
+// waves a SIMD the two come to as long as the step: one is hardly under the other, the waves spend a third of their time at waits.
+// Two tiles, because they and their state fit 168 registers, three blocks a CU; three tiles at two blocks a CU, with the scores of a
+// step computed under the weights of the one before, took 391 us where this takes 384 (8192 tokens, 32 heads over 8, window 4096:
+// 1075 TFLOP/s) and 293 where this takes 260 (e4m3, chunks of a long context). One tile for fewer rows: 128 registers, four blocks a
+// CU (e4m3: three, for the 48 KiB of LDS that a block takes). A third step in LDS, wave priorities and sums by matrix instructions
+// gave nothing.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int HALF = 8192;      // a step's K, or its V, in LDS
 
