@@ -672,8 +672,8 @@ def _check_window(what: str, q, k_cache, v_cache, block_tables, lens, scale, n_q
 
 def pick_window_splits(blocks: int, reach: int) -> int:
     """Splits of `paged_attn_decode_window` for `blocks` (sequence, 16 heads of a kv head) pairs that see up to `reach` keys each:
-    two blocks a CU; about 2048 keys a block at most, for even ends where blocks queue (1024 of 4096 keys: 1 split 261 us, 2 252;
-    512 of 1024 keys: 1 split 47 us, 2 50); 64 keys at least; 24 splits at most (each writes a part that the join reads)."""
+    two blocks a CU (an e4m3 cache: three fit); about 2048 keys a block at most, for even ends where blocks queue (1024 of 4096
+    keys: 1 split 261 us, 2 252; 512 of 1024 keys: 1 split 47 us, 2 50); 64 keys at least; 24 splits at most (each writes a part that the join reads)."""
     return max(1, min(max(-(-512 // max(1, blocks)), (reach + 1024) // 2048), reach // 64, 24))
 
 

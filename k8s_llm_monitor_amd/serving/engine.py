@@ -597,7 +597,8 @@ class Engine:
         g.replay()
 
     def warmup(self, buckets: Optional[Sequence[int]] = None) -> None:
-        """Capture the decode graphs ahead of traffic (padded rows only: no cache slot is written)."""
+        """Capture the decode graphs ahead of traffic (padded rows only: no cache slot is written). Those of launches with rules are
+        captured when the first such launch of a bucket comes, inside its step."""
         if not (self.on_gpu and self.cfg.use_graphs):
             return
         self._d_i32.zero_()
