@@ -727,7 +727,7 @@ class Engine:
         return {"model": self.mcfg.name, "params": self.mcfg.params(), "weight_bytes": self.model.weight_bytes(),
                 "kv_blocks": self.alloc.total, "kv_capacity_tokens": self.kv_capacity_tokens,
                 "kv_bytes": self.cache.nbytes, "max_num_seqs": self.cfg.max_num_seqs, "max_model_len": self.max_len,
-                "graphs": sorted(self._graphs), "device": str(self.device),
+                "graphs": sorted(self._graphs), "rule_graphs": sorted(self._rule_graphs), "device": str(self.device),
                 "decode_weights": "fp8 (W8A16, batch <= 128)" if self.model.fp8_decode else "bf16",
                 "window": self.mcfg.window, "sinks": self.mcfg.sinks,
                 "kv_cache_dtype": self.cfg.kv_cache_dtype, "mixed_batches": self.cfg.mixed_batches,

@@ -78,9 +78,11 @@ def test_a_smaller_cache_gives_its_memory_back():
     reqs = [eng.submit(list(range(1, 30 + i)), 30, TokenRules(repetition=1.5) if i else None) for i in range(3)]
     for _ in range(8):
         eng.step()
+    assert eng.describe()["rule_graphs"] == sorted(eng._rule_graphs) != []
     size, before = eng.cache.nbytes, torch.cuda.memory_reserved()
     eng.resize_cache(100)
     assert size > 1 << 30 and eng.cache.nbytes < size // 100 and before - torch.cuda.memory_reserved() > size * 9 // 10
+    assert eng.describe()["graphs"] == eng.describe()["rule_graphs"] == []
     while not eng.idle():
         eng.step()
     assert all(r.error is None and len(r.out) == 30 for r in reqs)
